@@ -11,17 +11,22 @@ import os
 import subprocess
 import sys
 import sysconfig
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 REPO_ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(REPO_ROOT, 'csrc')
 OUT = os.path.join(REPO_ROOT, 'kfac_amd', '_kfaccore.so')
 
 SOURCES = [
-    os.path.join(CSRC, 'syrk.hip'),
-    os.path.join(CSRC, 'gemm.hip'),
-    os.path.join(CSRC, 'eigh.hip'),
-    os.path.join(CSRC, 'chol.hip'),
-    os.path.join(CSRC, 'binding.cpp'),
+    os.path.join(CSRC, name)
+    for name in (
+        'syrk.hip',
+        'gemm.hip',
+        'eigh.hip',
+        'chol.hip',
+        'binding.cpp',
+    )
 ]
 HEADERS = [os.path.join(CSRC, 'common.h')]
 
@@ -54,14 +59,11 @@ def build(force: bool = False, arch: str = 'gfx950', verbose: bool = True) -> st
     lib_dirs = ce.library_paths('cuda')
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
 
-    cmd = [
-        'hipcc',
+    flags = [
         f'--offload-arch={arch}',
         '-O3',
         '-std=c++17',
         '-fPIC',
-        '-shared',
-        *SOURCES,
         *[f'-I{p}' for p in includes],
         '-D__HIP_PLATFORM_AMD__=1',
         '-DUSE_ROCM=1',
@@ -70,6 +72,13 @@ def build(force: bool = False, arch: str = 'gfx950', verbose: bool = True) -> st
         '-DTORCH_EXTENSION_NAME=_kfaccore',
         '-DTORCH_API_INCLUDE_EXTENSION_H',
         f'-D_GLIBCXX_USE_CXX11_ABI={abi}',
+    ]
+    # Packed fp32 instructions, which the compiler makes of ordinary float
+    # code, have given wrong results on this hardware now and then.
+    device_flags = [
+        '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops',
+    ]
+    link = [
         *[f'-L{p}' for p in lib_dirs],
         '-ltorch',
         '-ltorch_hip',
@@ -80,12 +89,39 @@ def build(force: bool = False, arch: str = 'gfx950', verbose: bool = True) -> st
         '-ltorch_python',
         '-lamdhip64',
         *[f'-Wl,-rpath,{p}' for p in lib_dirs],
-        '-o',
-        OUT,
     ]
-    if verbose:
-        print('[kfac_amd build]', ' '.join(cmd), file=sys.stderr)
-    subprocess.run(cmd, check=True)
+
+    def run(cmd: list[str]) -> None:
+        if verbose:
+            print('[kfac_amd build]', ' '.join(cmd), file=sys.stderr)
+        subprocess.run(cmd, check=True)
+
+    with tempfile.TemporaryDirectory() as tmp:
+        objects = [
+            os.path.join(tmp, os.path.basename(src) + '.o') for src in SOURCES
+        ]
+        commands = [
+            [
+                'hipcc',
+                '-c',
+                src,
+                *flags,
+                *(device_flags if src.endswith('.hip') else []),
+                '-o',
+                obj,
+            ]
+            for src, obj in zip(SOURCES, objects)
+        ]
+        with ThreadPoolExecutor(max_workers=8) as pool:
+            list(pool.map(run, commands))
+        # beside the library and renamed over it, so that a process that
+        # has it loaded keeps the old file
+        new = OUT + '.new'
+        run(
+            ['hipcc', f'--offload-arch={arch}', '-shared', *objects, *link,
+             '-o', new],
+        )
+        os.replace(new, OUT)
     return OUT
 
 
