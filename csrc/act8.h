@@ -1,0 +1,211 @@
+// Device helpers of the kernels that keep a transformer block's
+// activations in 8 bits (norm.hip, act8.hip, wgrad8.hip).
+//
+// The 8 bit form of a row: blocks of 64 consecutive values share one power
+// of two 2^e, the least with max |x| <= 127 * 2^e, and a value is stored as
+// the integer nearest to x / 2^e (ties to even). A power of two makes the
+// scaling and the way back exact, and code * 2^e has 7 significant bits, so
+// it is exact in bf16 too: the only rounding is the one to the code.
+// The exponent byte holds e + 127. It lies in [1, 248]: 2^-126 is the
+// least normal number, and 127 * 2^121 is the largest multiple that fp32
+// holds (larger values saturate to it). 255 marks a block with a NaN or an
+// infinity, all of which reads back as NaN.
+#pragma once
+
+#include "common.h"
+#include "training.h"
+
+namespace kfac {
+
+constexpr int kChunk = 8;    // values that a lane holds: 8 lanes a block
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+
+// 8 consecutive values. memcpy, because rows of an odd width start at any
+// multiple of the element: gfx950 loads and stores 16 bytes there as well.
+__device__ __forceinline__ void load8(const float* p, float v[8]) {
+  __builtin_memcpy(v, p, 32);
+}
+__device__ __forceinline__ void load8(const __hip_bfloat16* p, float v[8]) {
+  bf16x8 t;
+  __builtin_memcpy(&t, p, 16);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = (float)t[j];
+}
+__device__ __forceinline__ void load8(const __half* p, float v[8]) {
+  f16x8 t;
+  __builtin_memcpy(&t, p, 16);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = (float)t[j];
+}
+
+__device__ __forceinline__ void store8(float* p, const float v[8]) {
+  __builtin_memcpy(p, v, 32);
+}
+__device__ __forceinline__ void store8(__hip_bfloat16* p, const float v[8]) {
+  bf16x8 t;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) t[j] = (__bf16)v[j];
+  __builtin_memcpy(p, &t, 16);
+}
+__device__ __forceinline__ void store8(__half* p, const float v[8]) {
+  f16x8 t;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) t[j] = (_Float16)v[j];
+  __builtin_memcpy(p, &t, 16);
+}
+
+__device__ __forceinline__ float round_to(float v, const float*) { return v; }
+__device__ __forceinline__ float round_to(float v, const __hip_bfloat16*) {
+  return (float)(__bf16)v;
+}
+__device__ __forceinline__ float round_to(float v, const __half*) {
+  return (float)(_Float16)v;
+}
+
+__device__ __forceinline__ float load1(const float* p) { return *p; }
+__device__ __forceinline__ float load1(const __hip_bfloat16* p) {
+  return (float)*(const __bf16*)p;
+}
+__device__ __forceinline__ float load1(const __half* p) {
+  return (float)*(const _Float16*)p;
+}
+__device__ __forceinline__ void store1(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store1(__hip_bfloat16* p, float v) {
+  *(__bf16*)p = (__bf16)v;
+}
+__device__ __forceinline__ void store1(__half* p, float v) {
+  *(_Float16*)p = (_Float16)v;
+}
+
+// n of 8 values (n <= 0: none); the others read as 0 and are not written.
+template <typename T>
+__device__ __forceinline__ void load_chunk(const T* p, int n, float v[8]) {
+  if (n >= kChunk) {
+    load8(p, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) v[j] = j < n ? load1(p + j) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store_chunk(T* p, int n, const float v[8]) {
+  if (n >= kChunk) {
+    store8(p, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) {
+      if (j < n) store1(p + j, v[j]);
+    }
+  }
+}
+
+__device__ __forceinline__ void load_chunk(
+    const void* p,
+    int type,
+    long at,
+    int n,
+    float v[8]) {
+  if (type == kF32) {
+    load_chunk((const float*)p + at, n, v);
+  } else if (type == kBF16) {
+    load_chunk((const __hip_bfloat16*)p + at, n, v);
+  } else {
+    load_chunk((const __half*)p + at, n, v);
+  }
+}
+__device__ __forceinline__ void store_any(
+    void* p,
+    int type,
+    long at,
+    float v) {
+  if (type == kF32) {
+    store1((float*)p + at, v);
+  } else if (type == kBF16) {
+    store1((__hip_bfloat16*)p + at, v);
+  } else {
+    store1((__half*)p + at, v);
+  }
+}
+
+// Maximum over the 8 lanes of a block: two quad permutations and a
+// reversal of each half row, register moves without a trip through LDS.
+__device__ __forceinline__ unsigned max_of_block(unsigned m) {
+  unsigned o = __builtin_amdgcn_mov_dpp(m, 0xB1, 0xf, 0xf, true);
+  m = m > o ? m : o;
+  o = __builtin_amdgcn_mov_dpp(m, 0x4E, 0xf, 0xf, true);
+  m = m > o ? m : o;
+  o = __builtin_amdgcn_mov_dpp(m, 0x141, 0xf, 0xf, true);
+  return m > o ? m : o;
+}
+
+// Exponent byte of a block from the bits of max |x|. The bits order like
+// the numbers, infinities and NaN above all.
+__device__ __forceinline__ unsigned exponent_of(unsigned top) {
+  const unsigned p = top >> 23;
+  if (p == 255) return 255;
+  // 127 * 2^e = 1.984375 * 2^(e+6), whose mantissa bits are 0x7E0000
+  const int b = (int)p - 6 + ((top & 0x7FFFFF) > 0x7E0000 ? 1 : 0);
+  return b < 1 ? 1 : (b > 248 ? 248 : b);
+}
+
+__device__ __forceinline__ float scale_of(unsigned byte) {
+  return __uint_as_float(byte == 255 ? 0x7FC00000u : byte << 23);
+}
+
+// Packs the 8 values of each lane; all lanes of a block take part, those
+// behind the row's end with zeros. n: how many of the 8 are in the row.
+__device__ __forceinline__ void pack_chunk(
+    const float v[8],
+    int n,
+    int8_t* codes,
+    uint8_t* exponent,
+    bool first) {
+  unsigned top = 0;
+#pragma unroll
+  for (int j = 0; j < kChunk; ++j) {
+    const unsigned a = __float_as_uint(v[j]) & 0x7FFFFFFF;
+    top = top > a ? top : a;
+  }
+  const unsigned byte = exponent_of(max_of_block(top));
+  // 2^-e; a block that holds no number gets codes of 0
+  const float inv = __uint_as_float(byte == 255 ? 0u : (254 - byte) << 23);
+  unsigned char c[8];
+#pragma unroll
+  for (int j = 0; j < kChunk; ++j) {
+    float q = rintf(v[j] * inv);
+    q = fminf(fmaxf(q, -127.f), 127.f);
+    c[j] = byte == 255 ? 0 : (unsigned char)(int)q;
+  }
+  if (n >= kChunk) {
+    __builtin_memcpy(codes, c, 8);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) {
+      if (j < n) codes[j] = (int8_t)c[j];
+    }
+  }
+  if (first && n > 0) *exponent = (uint8_t)byte;
+}
+
+__device__ __forceinline__ void unpack_chunk(
+    const int8_t* codes,
+    unsigned byte,
+    int n,
+    float v[8]) {
+  const float s = scale_of(byte);
+  if (n >= kChunk) {
+    int8_t c[8];
+    __builtin_memcpy(c, codes, 8);
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) v[j] = (float)c[j] * s;
+  } else {
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) {
+      v[j] = j < n ? (float)codes[j] * s : 0.f;
+    }
+  }
+}
+
+}  // namespace kfac

@@ -1056,8 +1056,11 @@ torch::Tensor triu_unpack(torch::Tensor v, int64_t n) {
 
 }  // namespace
 
+void bind_training(pybind11::module& m);  // training.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "kfac_amd CDNA4 (gfx950) kernels";
+  bind_training(m);
   m.def("cov_linear", &cov_linear, "fused [a,1]^T[a,1] SYRK accumulation");
   m.def("cov_conv_a", &cov_conv_a, "fused im2col+SYRK A-factor accumulation");
   m.def("cov_conv_g", &cov_conv_g, "fused NCHW-transpose SYRK G-factor");

@@ -1,0 +1,615 @@
+// Layer norm of the rows of a matrix, forward and backward.
+//
+//   t = round(x + r)            the residual stream, kept in x's type
+//   h = (t - mean(t)) * rstd    rstd = 1 / sqrt(mean((t - mean)^2) + eps)
+//   y = round(h * w + b)
+//
+//   q  = dy * w
+//   dx = round(rstd * (q - mean(q) - h * mean(q * h)) + dt)
+//   dw = sum over rows of dy * h,   db = sum over rows of dy
+//
+// Both passes are bound by memory, so a row is read once: it stays in
+// registers between its sums and its outputs, 8 values a lane and chunk,
+// one wave a row up to 1024 values, 4 waves up to 4096, 16 up to 16384. The
+// variance is the mean of the centred squares of those registers, never a
+// difference of two large sums. The backward pass keeps dw and db of its
+// rows in registers too and writes one partial row a block; a second kernel
+// adds them in a fixed order, so that the gradients are the same from run
+// to run. Rows longer than 16384 take the kernels at the end of the file,
+// which read a row once for each of its sums.
+
+#include "act8.h"
+
+namespace kfac {
+
+namespace {
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+
+// Sum over the W waves of a row; every wave of the block calls it, as often
+// as the others. `at` alternates between two halves of `lds`, so that one
+// barrier a sum is enough.
+template <int W>
+__device__ __forceinline__ float row_sum(float v, float* lds, int& at) {
+  v = wave_sum(v);
+  if (W == 1) return v;
+  const int wave = threadIdx.x / kWave;
+  float* slot = lds + at * 16;
+  at ^= 1;
+  if (threadIdx.x % kWave == 0) slot[wave] = v;
+  __syncthreads();
+  const int first = wave / W * W;
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < W; ++i) s += slot[first + i];
+  return s;
+}
+
+struct Param {
+  const void* p;  // may be null
+  int type;
+};
+
+template <typename TX, typename TY>
+struct Forward {
+  const TX* x;
+  Param r, w, b;
+  TX* total;  // written if r is there
+  TY* y;
+  float* mean;
+  float* rstd;
+  int8_t* in_codes;  // may be null
+  uint8_t* in_exps;
+  int8_t* out_codes;  // may be null
+  uint8_t* out_exps;
+  long R;
+  int D;
+  int blocks;  // exponents a row
+  float eps;
+};
+
+template <typename TX, typename TY, int NCH, int W>
+__global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_fwd_kernel(
+    Forward<TX, TY> a) {
+  constexpr int G = W == 1 ? 4 : 1;  // rows of a block
+  __shared__ float lds[32];
+  int at = 0;
+  const int lane = threadIdx.x % (W * kWave);
+  const int group = threadIdx.x / (W * kWave);
+  float w[NCH][8], b[NCH][8];
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    const int col = (lane + i * W * kWave) * kChunk;
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) w[i][j] = 1.f, b[i][j] = 0.f;
+    if (a.w.p != nullptr) load_chunk(a.w.p, a.w.type, col, a.D - col, w[i]);
+    if (a.b.p != nullptr) load_chunk(a.b.p, a.b.type, col, a.D - col, b[i]);
+  }
+  for (long base = (long)blockIdx.x * G; base < a.R;
+       base += (long)gridDim.x * G) {
+    const long row = base + group;
+    const bool live = row < a.R;
+    const long start = row * a.D;
+    float t[NCH][8];
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int col = (lane + i * W * kWave) * kChunk;
+      const int n = live ? a.D - col : 0;
+      load_chunk(a.x + start + col, n, t[i]);
+      if (a.r.p != nullptr) {
+        float r[8];
+        load_chunk(a.r.p, a.r.type, start + col, n, r);
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) {
+          t[i][j] = round_to(t[i][j] + r[j], a.x);
+        }
+        store_chunk(a.total + start + col, n, t[i]);
+      }
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j) sum += t[i][j];
+    }
+    const float mean = row_sum<W>(sum, lds, at) / a.D;
+    float square = 0.f;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int n = a.D - (lane + i * W * kWave) * kChunk;
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j) {
+        const float c = j < n ? t[i][j] - mean : 0.f;
+        square += c * c;
+      }
+    }
+    const float var = row_sum<W>(square, lds, at) / a.D;
+    const float rstd = 1.f / sqrtf(var + a.eps);
+    if (live && lane == 0) {
+      a.mean[row] = mean;
+      a.rstd[row] = rstd;
+    }
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int chunk = lane + i * W * kWave;
+      const int col = chunk * kChunk;
+      const int n = live ? a.D - col : 0;
+      const long block = row * a.blocks + chunk / 8;
+      if (a.in_codes != nullptr) {
+        pack_chunk(
+            t[i], n, a.in_codes + start + col, a.in_exps + block,
+            chunk % 8 == 0);
+      }
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j) {
+        const float h = (t[i][j] - mean) * rstd;
+        t[i][j] = j < n ? round_to(h * w[i][j] + b[i][j], a.y) : 0.f;
+      }
+      store_chunk(a.y + start + col, n, t[i]);
+      if (a.out_codes != nullptr) {
+        pack_chunk(
+            t[i], n, a.out_codes + start + col, a.out_exps + block,
+            chunk % 8 == 0);
+      }
+    }
+  }
+}
+
+template <typename TX, typename TY>
+struct Backward {
+  const TY* dy;
+  const TX* x;  // null: codes and exps
+  const int8_t* codes;
+  const uint8_t* exps;
+  const float* mean;
+  const float* rstd;
+  Param w;
+  const TX* dt;  // may be null
+  TX* dx;
+  float* partial;  // [gridDim.x][2][D], null if no parameter has a gradient
+  long R;
+  int D;
+  int blocks;
+};
+
+template <typename TX, typename TY>
+__device__ __forceinline__ void load_kept(
+    const Backward<TX, TY>& a,
+    long row,
+    int col,
+    int n,
+    float v[8]) {
+  const long at = row * a.D + col;
+  if (a.x != nullptr) {
+    load_chunk(a.x + at, n, v);
+  } else if (n > 0) {
+    const unsigned byte = a.exps[row * a.blocks + col / kBlock8];
+    unpack_chunk(a.codes + at, byte, n, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) v[j] = 0.f;
+  }
+}
+
+template <typename TX, typename TY, int NCH, int W>
+__global__ __launch_bounds__(1024) void norm_bwd_kernel(Backward<TX, TY> a) {
+  constexpr int G = 16 / W;            // rows of a block
+  constexpr int kSpan = W * kWave * kChunk * NCH;  // columns of a group
+  __shared__ float lds[32];
+  __shared__ float parts[G > 1 ? G * kSpan : 1];
+  int at = 0;
+  const int lane = threadIdx.x % (W * kWave);
+  const int group = threadIdx.x / (W * kWave);
+  float w[NCH][8], dw[NCH][8], db[NCH][8];
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    const int col = (lane + i * W * kWave) * kChunk;
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) {
+      w[i][j] = 1.f;
+      dw[i][j] = db[i][j] = 0.f;
+    }
+    if (a.w.p != nullptr) load_chunk(a.w.p, a.w.type, col, a.D - col, w[i]);
+  }
+  for (long base = (long)blockIdx.x * G; base < a.R;
+       base += (long)gridDim.x * G) {
+    const long row = base + group;
+    const bool live = row < a.R;
+    const long start = row * a.D;
+    const float mean = live ? a.mean[row] : 0.f;
+    const float rstd = live ? a.rstd[row] : 0.f;
+    float q[NCH][8], h[NCH][8];
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int col = (lane + i * W * kWave) * kChunk;
+      const int n = live ? a.D - col : 0;
+      load_chunk(a.dy + start + col, n, q[i]);
+      load_kept(a, row, col, n, h[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int col = (lane + i * W * kWave) * kChunk;
+      const int n = live ? a.D - col : 0;
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j) {
+        h[i][j] = j < n ? (h[i][j] - mean) * rstd : 0.f;
+        dw[i][j] += q[i][j] * h[i][j];
+        db[i][j] += q[i][j];
+        q[i][j] *= w[i][j];
+        s1 += q[i][j];
+        s2 += q[i][j] * h[i][j];
+      }
+    }
+    s1 = row_sum<W>(s1, lds, at) / a.D;
+    s2 = row_sum<W>(s2, lds, at) / a.D;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int col = (lane + i * W * kWave) * kChunk;
+      const int n = live ? a.D - col : 0;
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j) {
+        q[i][j] = rstd * (q[i][j] - s1 - h[i][j] * s2);
+      }
+      if (a.dt != nullptr) {
+        float d[8];
+        load_chunk(a.dt + start + col, n, d);
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) q[i][j] += d[j];
+      }
+      store_chunk(a.dx + start + col, n, q[i]);
+    }
+  }
+  if (a.partial == nullptr) return;
+  float* mine = a.partial + (long)blockIdx.x * 2 * a.D;
+  if (G == 1) {
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int col = (lane + i * W * kWave) * kChunk;
+      store_chunk(mine + col, a.D - col, dw[i]);
+      store_chunk(mine + a.D + col, a.D - col, db[i]);
+    }
+    return;
+  }
+  // the groups' sums, added in the order of the groups
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int col = (lane + i * W * kWave) * kChunk;
+      store8(parts + group * kSpan + col, which ? db[i] : dw[i]);
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < a.D; c += 1024) {
+      float s = 0.f;
+#pragma unroll
+      for (int g = 0; g < G; ++g) s += parts[g * kSpan + c];
+      mine[which * a.D + c] = s;
+    }
+  }
+}
+
+// out[c] = sum over P of partial[p][which][c]: 64 columns a block, 16 waves
+// that each add every 16th row.
+__global__ __launch_bounds__(1024) void norm_param_kernel(
+    const float* __restrict__ partial,
+    int P,
+    int D,
+    void* dw,
+    int dw_type,
+    void* db,
+    int db_type) {
+  __shared__ float lds[16][kWave];
+  const int which = blockIdx.y;
+  void* out = which ? db : dw;
+  if (out == nullptr) return;
+  const int lane = threadIdx.x % kWave;
+  const int wave = threadIdx.x / kWave;
+  const int c = blockIdx.x * kWave + lane;
+  float s = 0.f;
+  if (c < D) {
+#pragma unroll 4
+    for (int p = wave; p < P; p += 16) {
+      s += partial[((long)p * 2 + which) * D + c];
+    }
+  }
+  lds[wave][lane] = s;
+  __syncthreads();
+  if (wave == 0 && c < D) {
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s += lds[i][lane];
+    store_any(out, which ? db_type : dw_type, c, s);
+  }
+}
+
+// -- rows longer than 16384: one block a row, which is read again from
+// memory (or the cache) for each of its sums -------------------------------
+
+constexpr int kLongSpan = 1024 * kChunk;
+
+template <typename TX, typename TY>
+__global__ __launch_bounds__(1024) void norm_fwd_long_kernel(
+    Forward<TX, TY> a) {
+  __shared__ float lds[32];
+  int at = 0;
+  const int first = threadIdx.x * kChunk;
+  const TX* kept = a.r.p != nullptr ? a.total : a.x;
+  for (long row = blockIdx.x; row < a.R; row += gridDim.x) {
+    const long start = row * a.D;
+    float sum = 0.f;
+    for (int c0 = 0; c0 < a.D; c0 += kLongSpan) {
+      const int col = c0 + first, n = a.D - col;
+      if (n <= 0) break;
+      float t[8];
+      load_chunk(a.x + start + col, n, t);
+      if (a.r.p != nullptr) {
+        float r[8];
+        load_chunk(a.r.p, a.r.type, start + col, n, r);
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) t[j] = round_to(t[j] + r[j], a.x);
+        // read again by the lane that wrote it
+        store_chunk(a.total + start + col, n, t);
+      }
+      float part = 0.f;
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j) part += t[j];
+      sum += part;
+    }
+    const float mean = row_sum<16>(sum, lds, at) / a.D;
+    float square = 0.f;
+    for (int c0 = 0; c0 < a.D; c0 += kLongSpan) {
+      const int col = c0 + first, n = a.D - col;
+      if (n <= 0) break;
+      float t[8], part = 0.f;
+      load_chunk(kept + start + col, n, t);
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j) {
+        const float c = j < n ? t[j] - mean : 0.f;
+        part += c * c;
+      }
+      square += part;
+    }
+    const float var = row_sum<16>(square, lds, at) / a.D;
+    const float rstd = 1.f / sqrtf(var + a.eps);
+    if (threadIdx.x == 0) {
+      a.mean[row] = mean;
+      a.rstd[row] = rstd;
+    }
+    // whole blocks of lanes: pack_chunk compares 8 neighbours
+    for (int c0 = 0; c0 < a.D; c0 += kLongSpan) {
+      const int col = c0 + first, n = a.D - col;
+      const int chunk = col / kChunk;
+      const long block = row * a.blocks + chunk / 8;
+      float t[8];
+      load_chunk(kept + start + col, n, t);
+      if (a.in_codes != nullptr) {
+        pack_chunk(
+            t, n, a.in_codes + start + col, a.in_exps + block, chunk % 8 == 0);
+      }
+      float w[8], b[8];
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j) w[j] = 1.f, b[j] = 0.f;
+      if (a.w.p != nullptr) load_chunk(a.w.p, a.w.type, col, n, w);
+      if (a.b.p != nullptr) load_chunk(a.b.p, a.b.type, col, n, b);
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j) {
+        t[j] = j < n ? round_to((t[j] - mean) * rstd * w[j] + b[j], a.y) : 0.f;
+      }
+      store_chunk(a.y + start + col, n, t);
+      if (a.out_codes != nullptr) {
+        pack_chunk(
+            t, n, a.out_codes + start + col, a.out_exps + block,
+            chunk % 8 == 0);
+      }
+    }
+  }
+}
+
+template <typename TX, typename TY>
+__global__ __launch_bounds__(1024) void norm_bwd_long_kernel(
+    Backward<TX, TY> a) {
+  __shared__ float lds[32];
+  int at = 0;
+  const int first = threadIdx.x * kChunk;
+  for (long row = blockIdx.x; row < a.R; row += gridDim.x) {
+    const long start = row * a.D;
+    const float mean = a.mean[row], rstd = a.rstd[row];
+    float s1 = 0.f, s2 = 0.f;
+    for (int pass = 0; pass < 2; ++pass) {
+      for (int c0 = 0; c0 < a.D; c0 += kLongSpan) {
+        const int col = c0 + first, n = a.D - col;
+        if (n <= 0) break;
+        float q[8], h[8], w[8];
+        load_chunk(a.dy + start + col, n, q);
+        load_kept(a, row, col, n, h);
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) w[j] = 1.f;
+        if (a.w.p != nullptr) load_chunk(a.w.p, a.w.type, col, n, w);
+        float p1 = 0.f, p2 = 0.f;
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) {
+          h[j] = j < n ? (h[j] - mean) * rstd : 0.f;
+          q[j] = j < n ? q[j] * w[j] : 0.f;
+          p1 += q[j];
+          p2 += q[j] * h[j];
+        }
+        if (pass == 0) {
+          s1 += p1;
+          s2 += p2;
+          continue;
+        }
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) q[j] = rstd * (q[j] - s1 - h[j] * s2);
+        if (a.dt != nullptr) {
+          float d[8];
+          load_chunk(a.dt + start + col, n, d);
+#pragma unroll
+          for (int j = 0; j < kChunk; ++j) q[j] += d[j];
+        }
+        store_chunk(a.dx + start + col, n, q);
+      }
+      if (pass == 0) {
+        s1 = row_sum<16>(s1, lds, at) / a.D;
+        s2 = row_sum<16>(s2, lds, at) / a.D;
+      }
+    }
+  }
+}
+
+// dw and db of long rows: a block takes 2048 columns, 8 a lane, and every
+// gridDim.y-th row.
+template <typename TX, typename TY>
+__global__ __launch_bounds__(256) void norm_bwd_long_param_kernel(
+    Backward<TX, TY> a) {
+  const int col = (blockIdx.x * 256 + threadIdx.x) * kChunk;
+  const int n = a.D - col;
+  if (n <= 0) return;
+  float dw[8] = {}, db[8] = {};
+  for (long row = blockIdx.y; row < a.R; row += gridDim.y) {
+    const float mean = a.mean[row], rstd = a.rstd[row];
+    float q[8], h[8];
+    load_chunk(a.dy + row * a.D + col, n, q);
+    load_kept(a, row, col, n, h);
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) {
+      dw[j] += j < n ? q[j] * ((h[j] - mean) * rstd) : 0.f;
+      db[j] += q[j];
+    }
+  }
+  float* mine = a.partial + (long)blockIdx.y * 2 * a.D;
+  store_chunk(mine + col, n, dw);
+  store_chunk(mine + a.D + col, n, db);
+}
+
+constexpr int kLongest = 16384;  // 16 waves x 2 chunks of 8 a lane
+constexpr int kLongSplit = 128;  // partial rows of the long form
+
+// Blocks of the backward kernel: what fills 256 compute units once, each
+// with the 16 waves that 128 registers a lane allow.
+int rows_of_block(int D) { return D <= 1024 ? 16 : D <= 4096 ? 4 : 1; }
+
+}  // namespace
+
+int norm_bwd_partials(long R, int D) {
+  if (D > kLongest) return (int)(R < kLongSplit ? R : kLongSplit);
+  const long need = (R + rows_of_block(D) - 1) / rows_of_block(D);
+  return (int)(need < 256 ? need : 256);
+}
+
+template <typename TX, typename TY>
+hipError_t norm_fwd_t(
+    hipStream_t s,
+    const TX* x,
+    const void* r,
+    int r_type,
+    const void* w,
+    int w_type,
+    const void* b,
+    int b_type,
+    TX* total,
+    TY* y,
+    float* mean,
+    float* rstd,
+    int8_t* in_codes,
+    uint8_t* in_exps,
+    int8_t* out_codes,
+    uint8_t* out_exps,
+    long R,
+    int D,
+    float eps) {
+  Forward<TX, TY> a{x,        {r, r_type}, {w, w_type}, {b, b_type},
+                    total,    y,           mean,        rstd,
+                    in_codes, in_exps,     out_codes,   out_exps,
+                    R,        D,           ceil_div(D, kBlock8), eps};
+  if (D > kLongest) {
+    norm_fwd_long_kernel<TX, TY><<<(unsigned)(R < 65536 ? R : 65536), 1024, 0, s>>>(a);
+    return hipGetLastError();
+  }
+  // 8 waves a SIMD: 2048 blocks of 256 threads, 512 of 1024
+  const auto go = [&](auto kernel, int rows, int threads) {
+    const long need = (R + rows - 1) / rows;
+    const long most = 2048L * 256 / threads;
+    kernel<<<(unsigned)(need < most ? need : most), threads, 0, s>>>(a);
+    return hipGetLastError();
+  };
+  if (D <= 512) return go(norm_fwd_kernel<TX, TY, 1, 1>, 4, 256);
+  if (D <= 1024) return go(norm_fwd_kernel<TX, TY, 2, 1>, 4, 256);
+  if (D <= 2048) return go(norm_fwd_kernel<TX, TY, 1, 4>, 1, 256);
+  if (D <= 4096) return go(norm_fwd_kernel<TX, TY, 2, 4>, 1, 256);
+  if (D <= 8192) return go(norm_fwd_kernel<TX, TY, 1, 16>, 1, 1024);
+  return go(norm_fwd_kernel<TX, TY, 2, 16>, 1, 1024);
+}
+
+// partial: norm_bwd_partials(R, D) x 2 x D, or null (then dw and db too)
+template <typename TX, typename TY>
+hipError_t norm_bwd_t(
+    hipStream_t s,
+    const TY* dy,
+    const TX* x,
+    const int8_t* codes,
+    const uint8_t* exps,
+    const float* mean,
+    const float* rstd,
+    const void* w,
+    int w_type,
+    const TX* dt,
+    TX* dx,
+    float* partial,
+    void* dw,
+    int dw_type,
+    void* db,
+    int db_type,
+    long R,
+    int D) {
+  Backward<TX, TY> a{dy, x,  codes,   exps, mean, rstd, {w, w_type},
+                     dt, dx, partial, R,    D,    ceil_div(D, kBlock8)};
+  const int P = norm_bwd_partials(R, D);
+  if (D > kLongest) {
+    norm_bwd_long_kernel<TX, TY><<<(unsigned)(R < 65536 ? R : 65536), 1024, 0, s>>>(a);
+    KFAC_HIP_CHECK(hipGetLastError());
+    if (partial != nullptr) {
+      const dim3 grid(ceil_div(D, 256 * kChunk), P);
+      norm_bwd_long_param_kernel<TX, TY><<<grid, 256, 0, s>>>(a);
+      KFAC_HIP_CHECK(hipGetLastError());
+    }
+  } else {
+    const auto go = [&](auto kernel) {
+      kernel<<<P, 1024, 0, s>>>(a);
+      return hipGetLastError();
+    };
+    KFAC_HIP_CHECK(
+        D <= 512        ? go(norm_bwd_kernel<TX, TY, 1, 1>)
+            : D <= 1024 ? go(norm_bwd_kernel<TX, TY, 2, 1>)
+            : D <= 2048 ? go(norm_bwd_kernel<TX, TY, 1, 4>)
+            : D <= 4096 ? go(norm_bwd_kernel<TX, TY, 2, 4>)
+            : D <= 8192 ? go(norm_bwd_kernel<TX, TY, 1, 16>)
+                        : go(norm_bwd_kernel<TX, TY, 2, 16>));
+  }
+  if (partial == nullptr) return hipSuccess;
+  norm_param_kernel<<<dim3(ceil_div(D, kWave), 2), 1024, 0, s>>>(
+      partial, P, D, dw, dw_type, db, db_type);
+  return hipGetLastError();
+}
+
+#define KFAC_NORM(TX, TY)                                                     \
+  template hipError_t norm_fwd_t<TX, TY>(                                     \
+      hipStream_t, const TX*, const void*, int, const void*, int,             \
+      const void*, int, TX*, TY*, float*, float*, int8_t*, uint8_t*, int8_t*, \
+      uint8_t*, long, int, float);                                            \
+  template hipError_t norm_bwd_t<TX, TY>(                                     \
+      hipStream_t, const TY*, const TX*, const int8_t*, const uint8_t*,       \
+      const float*, const float*, const void*, int, const TX*, TX*, float*,   \
+      void*, int, void*, int, long, int);
+KFAC_NORM(float, float)
+KFAC_NORM(float, __hip_bfloat16)
+KFAC_NORM(float, __half)
+KFAC_NORM(__hip_bfloat16, __hip_bfloat16)
+KFAC_NORM(__hip_bfloat16, float)
+KFAC_NORM(__half, __half)
+KFAC_NORM(__half, float)
+#undef KFAC_NORM
+
+}  // namespace kfac

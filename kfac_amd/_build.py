@@ -25,10 +25,16 @@ SOURCES = [
         'gemm.hip',
         'eigh.hip',
         'chol.hip',
+        'act8.hip',
+        'norm.hip',
+        'wgrad8.hip',
         'binding.cpp',
+        'training.cpp',
     )
 ]
-HEADERS = [os.path.join(CSRC, 'common.h')]
+HEADERS = [
+    os.path.join(CSRC, name) for name in ('common.h', 'act8.h', 'training.h')
+]
 
 
 def _needs_build() -> bool:

@@ -474,3 +474,21 @@ def triu_unpack(v: torch.Tensor, n: int, out: torch.Tensor | None = None) -> tor
         out.copy_(res)
         return out
     return res
+
+
+# The transformer block's training path (imported last: both modules take
+# the extension from this one).
+from kfac_amd.ops.activations import Activated8  # noqa: E402
+from kfac_amd.ops.activations import gelu8  # noqa: E402
+from kfac_amd.ops.activations import gelu8_backward  # noqa: E402
+from kfac_amd.ops.activations import gelu8_forward  # noqa: E402
+from kfac_amd.ops.activations import linear8  # noqa: E402
+from kfac_amd.ops.activations import pack8  # noqa: E402
+from kfac_amd.ops.activations import Packed8  # noqa: E402
+from kfac_amd.ops.activations import unpack8  # noqa: E402
+from kfac_amd.ops.activations import weight_grad8  # noqa: E402
+from kfac_amd.ops.norm import layer_norm  # noqa: E402
+from kfac_amd.ops.norm import layer_norm_backward  # noqa: E402
+from kfac_amd.ops.norm import layer_norm_forward  # noqa: E402
+from kfac_amd.ops.norm import Normed  # noqa: E402
+from kfac_amd.ops.norm import NormOutput  # noqa: E402

@@ -11,6 +11,8 @@ the HIP kernel does all of this in one pass over HBM.
 
 from __future__ import annotations
 
+import math
+
 import torch
 import torch.nn.functional as F
 
@@ -198,3 +200,137 @@ def triu_unpack(v: torch.Tensor, n: int) -> torch.Tensor:
     out[idx[0], idx[1]] = v
     out.t()[idx[0], idx[1]] = v
     return out
+
+
+# -- a transformer block's training path, activations kept in 8 bits --------
+
+BLOCK8 = 64  # consecutive values of a row that share a power of two
+
+
+def pack8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(codes, exponents) of the last dimension's blocks of 64 values.
+
+    value = code * 2^(exponent - 127), with the least power of two that
+    keeps the block within +-127; 255 marks a block that holds a NaN or an
+    infinity. See :func:`kfac_amd.ops.pack8`.
+    """
+    *lead, d = x.shape
+    blocks = -(-d // BLOCK8)
+    v = F.pad(x.to(torch.float32), (0, blocks * BLOCK8 - d))
+    v = v.view(*lead, blocks, BLOCK8)
+    top = v.abs().amax(-1)
+    bad = ~v.isfinite().all(-1)
+    part, power = torch.frexp(torch.where(bad, 0.0, top))  # part in [0.5, 1)
+    # 127 = 127/128 * 2^7
+    e = power.to(torch.int32) - 7 + (part > 127 / 128).to(torch.int32)
+    e = torch.where(part > 0, e, -126).clamp(-126, 121)
+    inv = torch.exp2(-e.to(torch.float64)).to(torch.float32)
+    codes = torch.round(v * inv.unsqueeze(-1)).clamp(-127, 127)
+    codes = torch.where(bad.unsqueeze(-1), 0.0, codes).to(torch.int8)
+    exps = torch.where(bad, 255, e + 127).to(torch.uint8)
+    return codes.view(*lead, blocks * BLOCK8)[..., :d].contiguous(), exps
+
+
+def unpack8(
+    codes: torch.Tensor,
+    exponents: torch.Tensor,
+    dtype: torch.dtype = torch.float32,
+) -> torch.Tensor:
+    """The values that 8 bit codes stand for."""
+    scale = torch.exp2(exponents.to(torch.float64) - 127).to(torch.float32)
+    scale = torch.where(exponents == 255, torch.nan, scale)
+    scale = scale.repeat_interleave(BLOCK8, dim=-1)[..., : codes.shape[-1]]
+    return (codes.to(torch.float32) * scale).to(dtype)
+
+
+def _gelu_gate(x: torch.Tensor) -> torch.Tensor:
+    u = math.sqrt(8 / math.pi) * (x + 0.044715 * x * x * x)
+    return 1 / (1 + torch.exp(-u))
+
+
+def gelu(x: torch.Tensor, approximate: str) -> torch.Tensor:
+    """x * P(x), P the normal distribution function or its tanh form."""
+    v = x.to(torch.float32)
+    if approximate == 'tanh':
+        return (v * _gelu_gate(v)).to(x.dtype)
+    return (v * 0.5 * torch.erfc(-v * math.sqrt(0.5))).to(x.dtype)
+
+
+def gelu_backward(
+    dy: torch.Tensor,
+    x: torch.Tensor,
+    approximate: str,
+) -> torch.Tensor:
+    """dy times GELU's slope at x, in dy's type."""
+    v = x.to(torch.float32)
+    if approximate == 'tanh':
+        p = _gelu_gate(v)
+        # p (1 - p) is 0 beyond |x| = 30, where x^2 may overflow
+        c = v.clamp(-30, 30)
+        slope = math.sqrt(8 / math.pi) * (1 + 3 * 0.044715 * c * c)
+        d = p + c * p * (1 - p) * slope
+    else:
+        d = 0.5 * torch.erfc(-v * math.sqrt(0.5)) + v * torch.exp(
+            -0.5 * v * v,
+        ) / math.sqrt(2 * math.pi)
+    return (dy.to(torch.float32) * d).to(dy.dtype)
+
+
+def weight_grad(
+    g: torch.Tensor,
+    a: torch.Tensor,
+    bias: bool,
+    dtype: torch.dtype,
+) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """(g^T a, column sums of g) over all rows, summed in fp32."""
+    g32 = g.to(torch.float32).reshape(-1, g.shape[-1])
+    a32 = a.to(torch.float32).reshape(-1, a.shape[-1])
+    db = g32.sum(0).to(dtype) if bias else None
+    return (g32.t() @ a32).to(dtype), db
+
+
+def layer_norm_forward(
+    x: torch.Tensor,
+    weight: torch.Tensor | None,
+    bias: torch.Tensor | None,
+    eps: float,
+    residual: torch.Tensor | None,
+    out_dtype: torch.dtype,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(y, total, mean, rstd); the statistics are flat, one a row."""
+    total = x
+    if residual is not None:
+        total = (x.to(torch.float32) + residual.to(torch.float32)).to(x.dtype)
+    t = total.to(torch.float32)
+    mean = t.mean(-1, keepdim=True)
+    var = (t - mean).square().mean(-1, keepdim=True)
+    rstd = 1 / torch.sqrt(var + eps)
+    y = (t - mean) * rstd
+    if weight is not None:
+        y = y * weight.to(torch.float32)
+    if bias is not None:
+        y = y + bias.to(torch.float32)
+    return y.to(out_dtype), total, mean.reshape(-1), rstd.reshape(-1)
+
+
+def layer_norm_backward(
+    dy: torch.Tensor,
+    total: torch.Tensor,
+    mean: torch.Tensor,
+    rstd: torch.Tensor,
+    weight: torch.Tensor | None,
+    grad_total: torch.Tensor | None,
+    dtype: torch.dtype,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dx, dweight, dbias), the parameters' gradients in fp32."""
+    d = dy.shape[-1]
+    g = dy.to(torch.float32).reshape(-1, d)
+    s = rstd.unsqueeze(-1)
+    h = (total.to(torch.float32).reshape(-1, d) - mean.unsqueeze(-1)) * s
+    q = g if weight is None else g * weight.to(torch.float32)
+    dx = s * (
+        q - q.mean(-1, keepdim=True) - h * (q * h).mean(-1, keepdim=True)
+    )
+    if grad_total is not None:
+        dx = dx + grad_total.to(torch.float32).reshape(-1, d)
+    return dx.to(dtype).view(dy.shape), (g * h).sum(0), g.sum(0)
