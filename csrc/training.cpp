@@ -356,10 +356,10 @@ std::tuple<Tensor, OptTensor> weight_grad8(
     if (want_bias) db = torch::zeros(bias_size, opts);
     return {torch::zeros(size, opts), db};
   }
-  const int parts = type_of(g.scalar_type()) == kfac::kF32 ? 3
-      : type_of(g.scalar_type()) == kfac::kF16             ? 2
-                                                           : 1;
-  const auto plan = kfac::wgrad8_plan(M, sg.D, sx.D, parts);
+  kfac::WGradPlan plan;
+  by_type(g.scalar_type(), [&](auto t) {
+    plan = kfac::wgrad8_plan<decltype(t)>(M, sg.D, sx.D);
+  });
   const long rows = (long)plan.splits * plan.tiles_k;
   auto dw = torch::empty(size, opts);
   if (want_bias) db = torch::empty(bias_size, opts);

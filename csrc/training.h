@@ -57,8 +57,8 @@ struct WGradPlan {
   int tiles_n, tiles_k;  // of the output
   long rows;             // tokens of a split
 };
-// parts: bf16 numbers that a gradient is the sum of (1, 2 or 3)
-WGradPlan wgrad8_plan(long M, int N, int K, int parts);
+template <typename TG>
+WGradPlan wgrad8_plan(long M, int N, int K);
 // sums: [splits][N][K]; bias: [splits * tiles_k][N], may be null
 template <typename TG>
 hipError_t wgrad8_t(
