@@ -12,6 +12,8 @@
 // infinity, all of which reads back as NaN.
 #pragma once
 
+#include <type_traits>
+
 #include "common.h"
 #include "training.h"
 
@@ -77,6 +79,51 @@ __device__ __forceinline__ void store1(__hip_bfloat16* p, float v) {
 }
 __device__ __forceinline__ void store1(__half* p, float v) {
   *(_Float16*)p = (_Float16)v;
+}
+
+typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
+
+__device__ __forceinline__ u32x4 load16(const void* p) {
+  u32x4 v;
+  __builtin_memcpy(&v, p, 16);
+  return v;
+}
+
+// 8 values as they are in memory, for loads long before their use.
+template <typename T>
+struct Raw {
+  u32x4 v[sizeof(T) / 2];
+
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = load16(p + i * 4);
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = (u32x4)(0u);
+  }
+  __device__ __forceinline__ void values(float f[8]) const {
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) {
+      const unsigned w = v[j * sizeof(T) / 16][j * sizeof(T) / 4 % 4];
+      if (sizeof(T) == 4) {
+        f[j] = __uint_as_float(w);
+      } else if (std::is_same<T, __hip_bfloat16>::value) {
+        f[j] = __uint_as_float(j % 2 ? w & 0xFFFF0000 : w << 16);
+      } else {
+        const unsigned short h = (unsigned short)(w >> j % 2 * 16);
+        f[j] = (float)__builtin_bit_cast(_Float16, h);
+      }
+    }
+  }
+};
+
+// base[at]: a 32 bit offset of a lane next to an address that its wave
+// shares, which is kept in scalar registers.
+template <typename T>
+__device__ __forceinline__ T* lane_ptr(T* base, unsigned at) {
+  using Byte = std::conditional_t<std::is_const<T>::value, const char, char>;
+  return (T*)((Byte*)base + at * (unsigned)sizeof(T));
 }
 
 // n of 8 values (n <= 0: none); the others read as 0 and are not written.
@@ -154,10 +201,39 @@ __device__ __forceinline__ float scale_of(unsigned byte) {
   return __uint_as_float(byte == 255 ? 0x7FC00000u : byte << 23);
 }
 
-// Packs the 8 values of each lane; all lanes of a block take part, those
-// behind the row's end with zeros. n: how many of the 8 are in the row.
+// Code B of the four in a word, as a float: one instruction.
+template <int B>
+__device__ __forceinline__ float code(unsigned word) {
+  float v;
+  if (B == 0) {
+    asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD "
+        "src0_sel:BYTE_0" : "=v"(v) : "v"(word));
+  } else if (B == 1) {
+    asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD "
+        "src0_sel:BYTE_1" : "=v"(v) : "v"(word));
+  } else if (B == 2) {
+    asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD "
+        "src0_sel:BYTE_2" : "=v"(v) : "v"(word));
+  } else {
+    asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD "
+        "src0_sel:BYTE_3" : "=v"(v) : "v"(word));
+  }
+  return v;
+}
+
+__device__ __forceinline__ void codes4(unsigned word, float s, float v[4]) {
+  v[0] = code<0>(word) * s;
+  v[1] = code<1>(word) * s;
+  v[2] = code<2>(word) * s;
+  v[3] = code<3>(word) * s;
+}
+
+// Packs the 8 values of each lane; all lanes of a block take part. Only the
+// values from `skip` on belong to the block, up to `n` (none if n <= skip):
+// the others are not looked at, and their codes not written.
 __device__ __forceinline__ void pack_chunk(
     const float v[8],
+    int skip,
     int n,
     int8_t* codes,
     uint8_t* exponent,
@@ -166,27 +242,39 @@ __device__ __forceinline__ void pack_chunk(
 #pragma unroll
   for (int j = 0; j < kChunk; ++j) {
     const unsigned a = __float_as_uint(v[j]) & 0x7FFFFFFF;
-    top = top > a ? top : a;
+    top = top > a || j < skip || j >= n ? top : a;
   }
   const unsigned byte = exponent_of(max_of_block(top));
   // 2^-e; a block that holds no number gets codes of 0
   const float inv = __uint_as_float(byte == 255 ? 0u : (254 - byte) << 23);
-  unsigned char c[8];
+  unsigned c[2] = {};
 #pragma unroll
   for (int j = 0; j < kChunk; ++j) {
-    float q = rintf(v[j] * inv);
-    q = fminf(fmaxf(q, -127.f), 127.f);
-    c[j] = byte == 255 ? 0 : (unsigned char)(int)q;
+    // a NaN becomes -127 and is dropped below
+    const float q = fminf(fmaxf(rintf(v[j] * inv), -127.f), 127.f);
+    c[j / 4] |= ((unsigned)(int)q & 255) << j % 4 * 8;
   }
-  if (n >= kChunk) {
+  if (byte == 255) c[0] = c[1] = 0;
+  if (skip == 0 && n >= kChunk) {
     __builtin_memcpy(codes, c, 8);
   } else {
 #pragma unroll
     for (int j = 0; j < kChunk; ++j) {
-      if (j < n) codes[j] = (int8_t)c[j];
+      if (j >= skip && j < n) codes[j] = (int8_t)(c[j / 4] >> j % 4 * 8);
     }
   }
-  if (first && n > 0) *exponent = (uint8_t)byte;
+  if (first && n > skip) *exponent = (uint8_t)byte;
+}
+
+__device__ __forceinline__ void unpack8(
+    const int8_t* codes,
+    unsigned byte,
+    float v[8]) {
+  const float s = scale_of(byte);
+  unsigned c[2];
+  __builtin_memcpy(c, codes, 8);
+  codes4(c[0], s, v);
+  codes4(c[1], s, v + 4);
 }
 
 __device__ __forceinline__ void unpack_chunk(
@@ -194,13 +282,10 @@ __device__ __forceinline__ void unpack_chunk(
     unsigned byte,
     int n,
     float v[8]) {
-  const float s = scale_of(byte);
   if (n >= kChunk) {
-    int8_t c[8];
-    __builtin_memcpy(c, codes, 8);
-#pragma unroll
-    for (int j = 0; j < kChunk; ++j) v[j] = (float)c[j] * s;
+    unpack8(codes, byte, v);
   } else {
+    const float s = scale_of(byte);
 #pragma unroll
     for (int j = 0; j < kChunk; ++j) {
       v[j] = j < n ? (float)codes[j] * s : 0.f;

@@ -43,7 +43,7 @@ __global__ __launch_bounds__(kThreads) void pack8_kernel(
   float v[8];
   load_chunk(x + at, t.n, v);
   pack_chunk(
-      v, t.n, codes + at, exps + t.row * blocks + t.chunk / 8,
+      v, 0, t.n, codes + at, exps + t.row * blocks + t.chunk / 8,
       t.chunk % 8 == 0);
 }
 
@@ -69,37 +69,57 @@ __global__ __launch_bounds__(kThreads) void unpack8_kernel(
 // GELU: y = x * P(x) with P the normal distribution function, or its tanh
 // form, a logistic gate: (1 + tanh u) / 2 = 1 / (1 + exp(-2u)).
 constexpr float kInvSqrt2Pi = 0.3989422804014327f;
+constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kGate = 1.5957691216057308f;  // 2 sqrt(2 / pi)
 constexpr float kCubic = 0.044715f;
 
-// P(x) and, in `density`, exp(-x^2/2) / sqrt(2 pi).
-__device__ __forceinline__ float normal_cdf(float x, float& density) {
-  density = expf(-0.5f * x * x) * kInvSqrt2Pi;
-  return 0.5f * erfcf(-x * 0.7071067811865476f);
+// P(-|x|) = exp(-x^2 / 2) * m(|x|), and the exponential. m, Mills' ratio
+// over sqrt(2 pi), is smooth and falls like 1 / |x|: a polynomial of degree
+// 7 in 1 / (1 + 0.34 |x|), fitted by reweighted least squares for an even
+// relative error up to |x| = 10, is off by 1.4e-7, and by 5e-7 when it is
+// evaluated in fp32. One exponential, one reciprocal and 14 other
+// operations; with the library's erfc these kernels were bound by
+// arithmetic (16384 x 4096 bf16: 147 us forward, 157 us backward).
+__device__ __forceinline__ float lower_tail(float x, float& exponential) {
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.34f, fabsf(x), 1.f));
+  float m = 0.0489479969f;
+  m = fmaf(m, t, -0.218984677f);
+  m = fmaf(m, t, 0.298419536f);
+  m = fmaf(m, t, -0.0649849661f);
+  m = fmaf(m, t, 0.176260347f);
+  m = fmaf(m, t, 0.123280336f);
+  m = fmaf(m, t, 0.137138441f);
+  m = fmaf(m, t, -7.70223557e-05f);
+  exponential = __builtin_amdgcn_exp2f(x * x * (-0.5f * kLog2e));
+  return exponential * m;
+}
+
+__device__ __forceinline__ float gate_of(float x) {
+  const float u = x * fmaf(kGate * kCubic * kLog2e, x * x, kGate * kLog2e);
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-u));
 }
 
 template <bool TANH>
 __device__ __forceinline__ float gelu_of(float x) {
-  if (TANH) {
-    const float u = kGate * (x + kCubic * x * x * x);
-    return x / (1.f + expf(-u));
-  }
-  float density;
-  return x * normal_cdf(x, density);
+  // below -100 the gate is 0: so is the result, at minus infinity too
+  if (TANH) return fmaxf(x, -100.f) * gate_of(x);
+  float e;
+  const float q = lower_tail(x, e);
+  return fmaf(-fminf(fabsf(x), 100.f), q, fmaxf(x, 0.f));
 }
 
 template <bool TANH>
 __device__ __forceinline__ float gelu_slope(float x) {
   if (TANH) {
-    const float p = 1.f / (1.f + expf(-kGate * (x + kCubic * x * x * x)));
+    const float p = gate_of(x);
     // p (1 - p) is 0 beyond |x| = 30, where x^2 may overflow
     const float c = fminf(fmaxf(x, -30.f), 30.f);
-    const float slope = kGate * (1.f + 3.f * kCubic * c * c);
-    return p + c * p * (1.f - p) * slope;
+    const float slope = kGate * fmaf(3.f * kCubic * c, c, 1.f);
+    return fmaf(c * p * (1.f - p), slope, p);
   }
-  float density;
-  const float p = normal_cdf(x, density);
-  return p + x * density;
+  float e;
+  const float q = lower_tail(x, e);
+  return fmaf(x * e, kInvSqrt2Pi, x < 0.f ? q : 1.f - q);
 }
 
 template <typename T, bool TANH>
@@ -123,13 +143,13 @@ __global__ __launch_bounds__(kThreads) void gelu8_fwd_kernel(
   float v[8];
   load_chunk(x + at, t.n, v);
   if (in_codes != nullptr) {
-    pack_chunk(v, t.n, in_codes + at, in_exps + block, first);
+    pack_chunk(v, 0, t.n, in_codes + at, in_exps + block, first);
   }
 #pragma unroll
   for (int j = 0; j < kChunk; ++j) v[j] = round_to(gelu_of<TANH>(v[j]), y);
   store_chunk(y + at, t.n, v);
   if (out_codes != nullptr) {
-    pack_chunk(v, t.n, out_codes + at, out_exps + block, first);
+    pack_chunk(v, 0, t.n, out_codes + at, out_exps + block, first);
   }
 }
 

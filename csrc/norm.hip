@@ -15,7 +15,7 @@
 // difference of two large sums. The backward pass keeps dw and db of its
 // rows in registers too and writes one partial row a block; a second kernel
 // adds them in a fixed order, so that the gradients are the same from run
-// to run. Rows longer than 16384 take the kernels at the end of the file,
+// to run. Rows longer than 16384 (or shorter than 8) take the kernels at the end of the file,
 // which read a row once for each of its sums.
 
 #include "act8.h"
@@ -24,10 +24,25 @@ namespace kfac {
 
 namespace {
 
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float v) {
+  return v + __int_as_float(__builtin_amdgcn_mov_dpp(
+                 __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+
+// Sum over a wave, the same bits in each lane: quads, halves and rows of 16
+// by register permutations, rows and halves of the wave by swaps.
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  return v;
+  v = add_dpp<0xB1>(v);
+  v = add_dpp<0x4E>(v);
+  v = add_dpp<0x141>(v);
+  v = add_dpp<0x140>(v);
+  const unsigned u = __float_as_uint(v);
+  const auto row = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  v = __uint_as_float(row[0]) + __uint_as_float(row[1]);
+  const unsigned w = __float_as_uint(v);
+  const auto half = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return __uint_as_float(half[0]) + __uint_as_float(half[1]);
 }
 
 // Sum over the W waves of a row; every wave of the block calls it, as often
@@ -54,6 +69,21 @@ struct Param {
   int type;
 };
 
+// 8 values from start + at on; the lanes of a wave share `start`.
+__device__ __forceinline__ void load_any(
+    const Param& a,
+    long start,
+    unsigned at,
+    float v[8]) {
+  if (a.type == kF32) {
+    load8(lane_ptr((const float*)a.p + start, at), v);
+  } else if (a.type == kBF16) {
+    load8(lane_ptr((const __hip_bfloat16*)a.p + start, at), v);
+  } else {
+    load8(lane_ptr((const __half*)a.p + start, at), v);
+  }
+}
+
 template <typename TX, typename TY>
 struct Forward {
   const TX* x;
@@ -72,85 +102,124 @@ struct Forward {
   float eps;
 };
 
-template <typename TX, typename TY, int NCH, int W>
-__global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_fwd_kernel(
+// A wave's row number, in a scalar register: rows are the same for a wave's
+// lanes, and addresses then cost no vector registers.
+__device__ __forceinline__ int group_of(int threads) {
+  return __builtin_amdgcn_readfirstlane(threadIdx.x / threads);
+}
+
+// The part of a row that a lane holds in chunk i of its NCH: 8 values from
+// `col`, of which those from `skip` on are its own. Where a row's length is
+// no multiple of 8 (ODD, 9 or more), the last lane takes the row's last 8
+// values, and its neighbour owns the first of them: both compute the same
+// results for these, and only sums have to leave one out.
+struct Part {
+  int chunk;
+  unsigned col;
+  int skip;
+  bool any;
+};
+
+template <bool ODD, int LANES>
+__device__ __forceinline__ Part part_of(int lane, int i, int D) {
+  Part p;
+  p.chunk = lane + i * LANES;
+  const int col = p.chunk * kChunk;
+  p.any = col < D;
+  p.skip = ODD && p.any && col > D - kChunk ? col - (D - kChunk) : 0;
+  p.col = p.any ? col - p.skip : 0;
+  return p;
+}
+
+// The lane's number, new to the compiler in each round of a loop: it would
+// keep a 64 bit address a lane for each tensor otherwise, and spill.
+__device__ __forceinline__ int fresh(int lane) {
+  asm volatile("" : "+v"(lane));
+  return lane;
+}
+
+template <typename TX, typename TY, int NCH, int W, bool ODD>
+__global__ __launch_bounds__(W == 1 ? 256 : W * kWave) void norm_fwd_kernel(
     Forward<TX, TY> a) {
+  constexpr int kLanes = W * kWave;
   constexpr int G = W == 1 ? 4 : 1;  // rows of a block
   __shared__ float lds[32];
   int at = 0;
-  const int lane = threadIdx.x % (W * kWave);
-  const int group = threadIdx.x / (W * kWave);
+  const int lane0 = threadIdx.x % kLanes;
+  const int group = group_of(kLanes);
+  const float mean_of = 1.f / a.D;
   float w[NCH][8], b[NCH][8];
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
-    const int col = (lane + i * W * kWave) * kChunk;
+    const Part p = part_of<ODD, kLanes>(lane0, i, a.D);
 #pragma unroll
     for (int j = 0; j < kChunk; ++j) w[i][j] = 1.f, b[i][j] = 0.f;
-    if (a.w.p != nullptr) load_chunk(a.w.p, a.w.type, col, a.D - col, w[i]);
-    if (a.b.p != nullptr) load_chunk(a.b.p, a.b.type, col, a.D - col, b[i]);
+    if (a.w.p != nullptr) load_any(a.w, 0, p.col, w[i]);
+    if (a.b.p != nullptr) load_any(a.b, 0, p.col, b[i]);
   }
   for (long base = (long)blockIdx.x * G; base < a.R;
        base += (long)gridDim.x * G) {
     const long row = base + group;
-    const bool live = row < a.R;
+    if (W == 1 && row >= a.R) return;
     const long start = row * a.D;
+    const int lane = fresh(lane0);
     float t[NCH][8];
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int col = (lane + i * W * kWave) * kChunk;
-      const int n = live ? a.D - col : 0;
-      load_chunk(a.x + start + col, n, t[i]);
+      const Part p = part_of<ODD, kLanes>(lane, i, a.D);
+      load8(lane_ptr(a.x + start, p.col), t[i]);
       if (a.r.p != nullptr) {
         float r[8];
-        load_chunk(a.r.p, a.r.type, start + col, n, r);
+        load_any(a.r, start, p.col, r);
 #pragma unroll
         for (int j = 0; j < kChunk; ++j) {
           t[i][j] = round_to(t[i][j] + r[j], a.x);
         }
-        store_chunk(a.total + start + col, n, t[i]);
+        if (p.any) store8(lane_ptr(a.total + start, p.col), t[i]);
       }
 #pragma unroll
-      for (int j = 0; j < kChunk; ++j) sum += t[i][j];
+      for (int j = 0; j < kChunk; ++j) {
+        sum += p.any && j >= p.skip ? t[i][j] : 0.f;
+      }
     }
     const float mean = row_sum<W>(sum, lds, at) / a.D;
     float square = 0.f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int n = a.D - (lane + i * W * kWave) * kChunk;
+      const Part p = part_of<ODD, kLanes>(lane, i, a.D);
 #pragma unroll
       for (int j = 0; j < kChunk; ++j) {
-        const float c = j < n ? t[i][j] - mean : 0.f;
+        const float c = p.any && j >= p.skip ? t[i][j] - mean : 0.f;
         square += c * c;
       }
     }
-    const float var = row_sum<W>(square, lds, at) / a.D;
-    const float rstd = 1.f / sqrtf(var + a.eps);
-    if (live && lane == 0) {
+    const float var = row_sum<W>(square, lds, at) * mean_of;
+    const float rstd = rsqrtf(var + a.eps);
+    if (lane == 0) {
       a.mean[row] = mean;
       a.rstd[row] = rstd;
     }
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int chunk = lane + i * W * kWave;
-      const int col = chunk * kChunk;
-      const int n = live ? a.D - col : 0;
-      const long block = row * a.blocks + chunk / 8;
+      const Part p = part_of<ODD, kLanes>(lane, i, a.D);
+      const long block = row * a.blocks;
+      const int n = p.any ? kChunk : 0;
       if (a.in_codes != nullptr) {
         pack_chunk(
-            t[i], n, a.in_codes + start + col, a.in_exps + block,
-            chunk % 8 == 0);
+            t[i], p.skip, n, lane_ptr(a.in_codes + start, p.col),
+            lane_ptr(a.in_exps + block, p.chunk / 8), p.chunk % 8 == 0);
       }
 #pragma unroll
       for (int j = 0; j < kChunk; ++j) {
         const float h = (t[i][j] - mean) * rstd;
-        t[i][j] = j < n ? round_to(h * w[i][j] + b[i][j], a.y) : 0.f;
+        t[i][j] = round_to(h * w[i][j] + b[i][j], a.y);
       }
-      store_chunk(a.y + start + col, n, t[i]);
+      if (p.any) store8(lane_ptr(a.y + start, p.col), t[i]);
       if (a.out_codes != nullptr) {
         pack_chunk(
-            t[i], n, a.out_codes + start + col, a.out_exps + block,
-            chunk % 8 == 0);
+            t[i], p.skip, n, lane_ptr(a.out_codes + start, p.col),
+            lane_ptr(a.out_exps + block, p.chunk / 8), p.chunk % 8 == 0);
       }
     }
   }
@@ -192,73 +261,103 @@ __device__ __forceinline__ void load_kept(
   }
 }
 
-template <typename TX, typename TY, int NCH, int W>
+template <typename TX, typename TY, int NCH, int W, bool ODD, bool KEPT8>
 __global__ __launch_bounds__(1024) void norm_bwd_kernel(Backward<TX, TY> a) {
-  constexpr int G = 16 / W;            // rows of a block
-  constexpr int kSpan = W * kWave * kChunk * NCH;  // columns of a group
+  constexpr int kLanes = W * kWave;
+  constexpr int G = 16 / W;                     // rows of a block
+  constexpr int kSpan = kLanes * kChunk * NCH;  // columns of a group
   __shared__ float lds[32];
   __shared__ float parts[G > 1 ? G * kSpan : 1];
   int at = 0;
-  const int lane = threadIdx.x % (W * kWave);
-  const int group = threadIdx.x / (W * kWave);
+  const int lane0 = threadIdx.x % kLanes;
+  const int group = group_of(kLanes);
+  const float mean_of = 1.f / a.D;
   float w[NCH][8], dw[NCH][8], db[NCH][8];
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
-    const int col = (lane + i * W * kWave) * kChunk;
+    const Part p = part_of<ODD, kLanes>(lane0, i, a.D);
 #pragma unroll
     for (int j = 0; j < kChunk; ++j) {
       w[i][j] = 1.f;
       dw[i][j] = db[i][j] = 0.f;
     }
-    if (a.w.p != nullptr) load_chunk(a.w.p, a.w.type, col, a.D - col, w[i]);
+    if (a.w.p != nullptr) load_any(a.w, 0, p.col, w[i]);
   }
   for (long base = (long)blockIdx.x * G; base < a.R;
        base += (long)gridDim.x * G) {
-    const long row = base + group;
-    const bool live = row < a.R;
+    const bool live = base + group < a.R;
+    if (W == 1 && !live) break;
+    // a group without a row takes part in the barriers, with row 0
+    const long row = live ? base + group : 0;
     const long start = row * a.D;
-    const float mean = live ? a.mean[row] : 0.f;
-    const float rstd = live ? a.rstd[row] : 0.f;
-    float q[NCH][8], h[NCH][8];
+    const int lane = fresh(lane0);
+    const float mean = a.mean[row], rstd = a.rstd[row];
+    Raw<TY> dy[NCH];
+    Raw<TX> dt[NCH];
+    float h[NCH][8];
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int col = (lane + i * W * kWave) * kChunk;
-      const int n = live ? a.D - col : 0;
-      load_chunk(a.dy + start + col, n, q[i]);
-      load_kept(a, row, col, n, h[i]);
+      const Part p = part_of<ODD, kLanes>(lane, i, a.D);
+      dy[i].load(lane_ptr(a.dy + start, p.col));
+      if (KEPT8) {
+        const uint8_t* e = a.exps + row * a.blocks;
+        const int8_t* c = lane_ptr(a.codes + start, p.col);
+        unpack8(c, *lane_ptr(e, p.col / kBlock8), h[i]);
+        if (ODD && p.skip > 0) {
+          // the last lane's own values may be in the next block
+          float own[8];
+          unpack8(c, *lane_ptr(e, p.chunk / 8), own);
+#pragma unroll
+          for (int j = 0; j < kChunk; ++j) {
+            h[i][j] = j < p.skip ? h[i][j] : own[j];
+          }
+        }
+      } else {
+        load8(lane_ptr(a.x + start, p.col), h[i]);
+      }
+    }
+    if (a.dt != nullptr) {
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        const Part p = part_of<ODD, kLanes>(lane, i, a.D);
+        dt[i].load(lane_ptr(a.dt + start, p.col));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) dt[i].clear();
     }
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int col = (lane + i * W * kWave) * kChunk;
-      const int n = live ? a.D - col : 0;
+      const Part p = part_of<ODD, kLanes>(lane, i, a.D);
+      float g[8];
+      dy[i].values(g);
 #pragma unroll
       for (int j = 0; j < kChunk; ++j) {
-        h[i][j] = j < n ? (h[i][j] - mean) * rstd : 0.f;
-        dw[i][j] += q[i][j] * h[i][j];
-        db[i][j] += q[i][j];
-        q[i][j] *= w[i][j];
-        s1 += q[i][j];
-        s2 += q[i][j] * h[i][j];
+        h[i][j] = (h[i][j] - mean) * rstd;
+        const float own = live && p.any && j >= p.skip ? g[j] : 0.f;
+        const float product = own * h[i][j];
+        dw[i][j] += product;
+        db[i][j] += own;
+        // added here, not behind the stores: both terms would be kept
+        asm volatile("" : "+v"(dw[i][j]), "+v"(db[i][j]));
+        s1 += own * w[i][j];
+        s2 += product * w[i][j];
       }
     }
-    s1 = row_sum<W>(s1, lds, at) / a.D;
-    s2 = row_sum<W>(s2, lds, at) / a.D;
+    s1 = row_sum<W>(s1, lds, at) * mean_of;
+    s2 = row_sum<W>(s2, lds, at) * mean_of;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int col = (lane + i * W * kWave) * kChunk;
-      const int n = live ? a.D - col : 0;
+      const Part p = part_of<ODD, kLanes>(lane, i, a.D);
+      float g[8], d[8];
+      dy[i].values(g);
+      dt[i].values(d);
 #pragma unroll
       for (int j = 0; j < kChunk; ++j) {
-        q[i][j] = rstd * (q[i][j] - s1 - h[i][j] * s2);
+        d[j] += rstd * (g[j] * w[i][j] - s1 - h[i][j] * s2);
       }
-      if (a.dt != nullptr) {
-        float d[8];
-        load_chunk(a.dt + start + col, n, d);
-#pragma unroll
-        for (int j = 0; j < kChunk; ++j) q[i][j] += d[j];
-      }
-      store_chunk(a.dx + start + col, n, q[i]);
+      if (live && p.any) store8(lane_ptr(a.dx + start, p.col), d);
     }
   }
   if (a.partial == nullptr) return;
@@ -266,9 +365,14 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(Backward<TX, TY> a) {
   if (G == 1) {
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int col = (lane + i * W * kWave) * kChunk;
-      store_chunk(mine + col, a.D - col, dw[i]);
-      store_chunk(mine + a.D + col, a.D - col, db[i]);
+      const Part p = part_of<ODD, kLanes>(lane0, i, a.D);
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j) {
+        if (p.any && j >= p.skip) {
+          mine[p.col + j] = dw[i][j];
+          mine[a.D + p.col + j] = db[i][j];
+        }
+      }
     }
     return;
   }
@@ -278,8 +382,13 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(Backward<TX, TY> a) {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int col = (lane + i * W * kWave) * kChunk;
-      store8(parts + group * kSpan + col, which ? db[i] : dw[i]);
+      const Part p = part_of<ODD, kLanes>(lane0, i, a.D);
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j) {
+        if (p.any && j >= p.skip) {
+          parts[group * kSpan + p.col + j] = which ? db[i][j] : dw[i][j];
+        }
+      }
     }
     __syncthreads();
     for (int c = threadIdx.x; c < a.D; c += 1024) {
@@ -373,7 +482,7 @@ __global__ __launch_bounds__(1024) void norm_fwd_long_kernel(
       square += part;
     }
     const float var = row_sum<16>(square, lds, at) / a.D;
-    const float rstd = 1.f / sqrtf(var + a.eps);
+    const float rstd = rsqrtf(var + a.eps);
     if (threadIdx.x == 0) {
       a.mean[row] = mean;
       a.rstd[row] = rstd;
@@ -387,7 +496,8 @@ __global__ __launch_bounds__(1024) void norm_fwd_long_kernel(
       load_chunk(kept + start + col, n, t);
       if (a.in_codes != nullptr) {
         pack_chunk(
-            t, n, a.in_codes + start + col, a.in_exps + block, chunk % 8 == 0);
+            t, 0, n, a.in_codes + start + col, a.in_exps + block,
+            chunk % 8 == 0);
       }
       float w[8], b[8];
 #pragma unroll
@@ -401,7 +511,7 @@ __global__ __launch_bounds__(1024) void norm_fwd_long_kernel(
       store_chunk(a.y + start + col, n, t);
       if (a.out_codes != nullptr) {
         pack_chunk(
-            t, n, a.out_codes + start + col, a.out_exps + block,
+            t, 0, n, a.out_codes + start + col, a.out_exps + block,
             chunk % 8 == 0);
       }
     }
@@ -484,17 +594,38 @@ __global__ __launch_bounds__(256) void norm_bwd_long_param_kernel(
   store_chunk(mine + a.D + col, n, db);
 }
 
-constexpr int kLongest = 16384;  // 16 waves x 2 chunks of 8 a lane
+// 16 waves x 2 chunks of 8 a lane. Rows of 1 to 7 values, of which no lane
+// can take 8, go the way of the longer ones too.
+bool is_long(int D) { return D > 16384 || D < kChunk; }
 constexpr int kLongSplit = 128;  // partial rows of the long form
 
 // Blocks of the backward kernel: what fills 256 compute units once, each
 // with the 16 waves that 128 registers a lane allow.
 int rows_of_block(int D) { return D <= 1024 ? 16 : D <= 4096 ? 4 : 1; }
 
+// Calls fn with the kernel's template parameters (chunks of a lane, waves of
+// a row, odd length) as types.
+template <typename Fn>
+hipError_t by_width(int D, Fn fn) {
+  const auto go = [&](auto odd) {
+    using I1 = std::integral_constant<int, 1>;
+    using I2 = std::integral_constant<int, 2>;
+    using I4 = std::integral_constant<int, 4>;
+    using I16 = std::integral_constant<int, 16>;
+    return D <= 512 ? fn(I1(), I1(), odd)
+        : D <= 1024 ? fn(I2(), I1(), odd)
+        : D <= 2048 ? fn(I1(), I4(), odd)
+        : D <= 4096 ? fn(I2(), I4(), odd)
+        : D <= 8192 ? fn(I1(), I16(), odd)
+                    : fn(I2(), I16(), odd);
+  };
+  return D % kChunk ? go(std::true_type()) : go(std::false_type());
+}
+
 }  // namespace
 
 int norm_bwd_partials(long R, int D) {
-  if (D > kLongest) return (int)(R < kLongSplit ? R : kLongSplit);
+  if (is_long(D)) return (int)(R < kLongSplit ? R : kLongSplit);
   const long need = (R + rows_of_block(D) - 1) / rows_of_block(D);
   return (int)(need < 256 ? need : 256);
 }
@@ -524,23 +655,20 @@ hipError_t norm_fwd_t(
                     total,    y,           mean,        rstd,
                     in_codes, in_exps,     out_codes,   out_exps,
                     R,        D,           ceil_div(D, kBlock8), eps};
-  if (D > kLongest) {
+  if (is_long(D)) {
     norm_fwd_long_kernel<TX, TY><<<(unsigned)(R < 65536 ? R : 65536), 1024, 0, s>>>(a);
     return hipGetLastError();
   }
   // 8 waves a SIMD: 2048 blocks of 256 threads, 512 of 1024
-  const auto go = [&](auto kernel, int rows, int threads) {
-    const long need = (R + rows - 1) / rows;
+  return by_width(D, [&](auto nch, auto waves, auto odd) {
+    constexpr int W = decltype(waves)::value;
+    constexpr int threads = W == 1 ? 256 : W * kWave;
+    const long need = W == 1 ? (R + 3) / 4 : R;
     const long most = 2048L * 256 / threads;
-    kernel<<<(unsigned)(need < most ? need : most), threads, 0, s>>>(a);
+    norm_fwd_kernel<TX, TY, decltype(nch)::value, W, decltype(odd)::value>
+        <<<(unsigned)(need < most ? need : most), threads, 0, s>>>(a);
     return hipGetLastError();
-  };
-  if (D <= 512) return go(norm_fwd_kernel<TX, TY, 1, 1>, 4, 256);
-  if (D <= 1024) return go(norm_fwd_kernel<TX, TY, 2, 1>, 4, 256);
-  if (D <= 2048) return go(norm_fwd_kernel<TX, TY, 1, 4>, 1, 256);
-  if (D <= 4096) return go(norm_fwd_kernel<TX, TY, 2, 4>, 1, 256);
-  if (D <= 8192) return go(norm_fwd_kernel<TX, TY, 1, 16>, 1, 1024);
-  return go(norm_fwd_kernel<TX, TY, 2, 16>, 1, 1024);
+  });
 }
 
 // partial: norm_bwd_partials(R, D) x 2 x D, or null (then dw and db too)
@@ -567,7 +695,7 @@ hipError_t norm_bwd_t(
   Backward<TX, TY> a{dy, x,  codes,   exps, mean, rstd, {w, w_type},
                      dt, dx, partial, R,    D,    ceil_div(D, kBlock8)};
   const int P = norm_bwd_partials(R, D);
-  if (D > kLongest) {
+  if (is_long(D)) {
     norm_bwd_long_kernel<TX, TY><<<(unsigned)(R < 65536 ? R : 65536), 1024, 0, s>>>(a);
     KFAC_HIP_CHECK(hipGetLastError());
     if (partial != nullptr) {
@@ -576,17 +704,16 @@ hipError_t norm_bwd_t(
       KFAC_HIP_CHECK(hipGetLastError());
     }
   } else {
-    const auto go = [&](auto kernel) {
-      kernel<<<P, 1024, 0, s>>>(a);
+    KFAC_HIP_CHECK(by_width(D, [&](auto nch, auto waves, auto odd) {
+      constexpr int N = decltype(nch)::value, W = decltype(waves)::value;
+      constexpr bool ODD = decltype(odd)::value;
+      if (x != nullptr) {
+        norm_bwd_kernel<TX, TY, N, W, ODD, false><<<P, 1024, 0, s>>>(a);
+      } else {
+        norm_bwd_kernel<TX, TY, N, W, ODD, true><<<P, 1024, 0, s>>>(a);
+      }
       return hipGetLastError();
-    };
-    KFAC_HIP_CHECK(
-        D <= 512        ? go(norm_bwd_kernel<TX, TY, 1, 1>)
-            : D <= 1024 ? go(norm_bwd_kernel<TX, TY, 2, 1>)
-            : D <= 2048 ? go(norm_bwd_kernel<TX, TY, 1, 4>)
-            : D <= 4096 ? go(norm_bwd_kernel<TX, TY, 2, 4>)
-            : D <= 8192 ? go(norm_bwd_kernel<TX, TY, 1, 16>)
-                        : go(norm_bwd_kernel<TX, TY, 2, 16>));
+    }));
   }
   if (partial == nullptr) return hipSuccess;
   norm_param_kernel<<<dim3(ceil_div(D, kWave), 2), 1024, 0, s>>>(

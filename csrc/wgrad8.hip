@@ -19,8 +19,6 @@
 // fill the card; the splits' fp32 sums are added by a second kernel in a
 // fixed order.
 
-#include <type_traits>
-
 #include "act8.h"
 
 namespace kfac {
@@ -97,36 +95,6 @@ __device__ __forceinline__ unsigned high_halves(float lo, float hi) {
   return __builtin_amdgcn_perm(
       __float_as_uint(hi), __float_as_uint(lo), 0x07060302);
 }
-
-typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
-
-__device__ __forceinline__ u32x4 load16(const void* p) {
-  u32x4 v;
-  __builtin_memcpy(&v, p, 16);
-  return v;
-}
-
-// 8 gradients as they are in memory.
-template <typename TG>
-struct Raw {
-  u32x4 v[sizeof(TG) / 2];
-
-  __device__ __forceinline__ void load(const TG* p) {
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(TG) / 2; ++i) v[i] = load16(p + i * 4);
-  }
-  __device__ __forceinline__ void values(float f[8]) const {
-#pragma unroll
-    for (int j = 0; j < kChunk; ++j) {
-      if (sizeof(TG) == 4) {
-        f[j] = __uint_as_float(v[j / 4][j % 4]);
-      } else {
-        const unsigned short h = (unsigned short)(v[0][j / 2] >> j % 2 * 16);
-        f[j] = (float)__builtin_bit_cast(_Float16, h);
-      }
-    }
-  }
-};
 
 // Takes the leading 8 bits of each of 8 values off as bf16. Cut, not
 // rounded: the rest is exact, and nothing overflows. An infinity leaves
@@ -220,13 +188,11 @@ __global__ __launch_bounds__(WN * WK * kWave) void wgrad8_kernel(WGrad a) {
     const float s = scale_of(xe[i]);
     unsigned v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      // codes as bytes from 0 to 255, less 128: exact, as the result is
-      const unsigned c = xv[i][j / 2] ^ 0x80808080;
-      const int b = j % 2 * 16;
-      v[j] = high_halves(
-          fmaf((float)(c >> b & 255), s, -128.f * s),
-          fmaf((float)(c >> (b + 8) & 255), s, -128.f * s));
+    for (int j = 0; j < 4; ++j) {
+      float f[4];
+      codes4(xv[i][j], s, f);
+      v[2 * j] = high_halves(f[0], f[1]);
+      v[2 * j + 1] = high_halves(f[2], f[3]);
     }
     const int row = x_row + i * kXDown, chunk = x_col / 8;
     __builtin_memcpy(xl + slot<BK>(row, chunk) * 8, v, 16);
