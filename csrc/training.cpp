@@ -367,7 +367,9 @@ std::tuple<Tensor, OptTensor> weight_grad8(
   const bool direct = plan.splits == 1 && dtype == torch::kFloat32;
   const bool bias_direct = rows == 1 && dtype == torch::kFloat32;
   Tensor sums = dw, bias = want_bias ? *db : Tensor();
-  if (!direct) sums = torch::empty({plan.splits * N * K}, f32);
+  if (!direct) {
+    sums = torch::empty({plan.splits * N * K}, f32);
+  }
   if (want_bias && !bias_direct) bias = torch::empty({rows * N}, f32);
   const auto stream = stream_of(g);
   by_type(g.scalar_type(), [&](auto t) {
@@ -379,16 +381,12 @@ std::tuple<Tensor, OptTensor> weight_grad8(
         sums.data_ptr<float>(),
         want_bias ? bias.data_ptr<float>() : nullptr));
   });
-  if (!direct) {
-    CHECK_OK(kfac::wgrad8_add(
-        stream, sums.data_ptr<float>(), plan.splits, N * K, dw.data_ptr(),
-        type_of(dtype)));
-  }
-  if (want_bias && !bias_direct) {
-    CHECK_OK(kfac::wgrad8_add(
-        stream, bias.data_ptr<float>(), (int)rows, N, db->data_ptr(),
-        type_of(dtype)));
-  }
+  const bool add_bias = want_bias && !bias_direct;
+  CHECK_OK(kfac::wgrad8_add(
+      stream, sums.data_ptr<float>(), plan.splits, N * K,
+      direct ? nullptr : dw.data_ptr(),
+      add_bias ? bias.data_ptr<float>() : nullptr, (int)rows, N,
+      add_bias ? db->data_ptr() : nullptr, type_of(dtype)));
   return {dw, db};
 }
 

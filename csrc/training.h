@@ -53,6 +53,7 @@ hipError_t norm_bwd_t(
 
 // How a weight gradient is cut into blocks.
 struct WGradPlan {
+  bool large;            // tiles
   int splits;            // of the tokens
   int tiles_n, tiles_k;  // of the output
   long rows;             // tokens of a split
@@ -64,8 +65,11 @@ template <typename TG>
 hipError_t wgrad8_t(
     hipStream_t, const TG* g, const int8_t* codes, const uint8_t* exps,
     long M, int N, int K, const WGradPlan& plan, float* sums, float* bias);
-// out[i] = sum over s of sums[s][i], i < n
+// out[i] = sum over s < splits of sums[s][i], i < n, and the same for the
+// bias; either output may be null
 hipError_t wgrad8_add(
-    hipStream_t, const float* sums, int S, long n, void* out, int type);
+    hipStream_t, const float* sums, int splits, long n, void* out,
+    const float* bias_sums, int bias_rows, long bias_n, void* bias_out,
+    int type);
 
 }  // namespace kfac

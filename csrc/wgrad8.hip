@@ -205,51 +205,44 @@ __global__ __launch_bounds__(WN * WK * kWave) void wgrad8_kernel(WGrad a) {
   for (int i = 0; i < FN; ++i) g_frag[i] = fragment_at<BN>(wn + i * 32, lane);
 #pragma unroll
   for (int j = 0; j < FK; ++j) x_frag[j] = fragment_at<BK>(wk + j * 32, lane);
-  // The products of a stage's image; other(r) runs between them.
-  const auto products = [&](const short* gl, int stage, auto other) {
-    const short* xl = gl + NP * BM * BN;
-    if (a.bias != nullptr && stage % a.tiles_k == tile.k) {
-      // the tiles of a row share the work of the bias's sum
+  constexpr int kQ = kSteps * NP;  // fragments of g and a 16 token step
+  static_assert(kSteps % 2 == 0, "fragments alternate");
+  bf16x8 f[2][FN], x[2][FK];
+  const auto read = [&](const short* gl, int q) {
+    const int r = q / NP, p = q % NP;
 #pragma unroll
-      for (int i = 0; i < GC * NP; ++i) {
-        const int row = g_row + i % GC * kGDown;
-        float v[8];
-        load8(
-            (const __hip_bfloat16*)gl + i / GC * BM * BN +
-                slot<BN>(row, g_col / 8) * 8,
-            v);
+    for (int j = 0; p == 0 && j < FK; ++j) {
+      x[r & 1][j] =
+          fragment<BK>(gl + NP * BM * BN + x_frag[j] + r * 16 * BK);
+    }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) bias[j] += v[j];
+    for (int i = 0; i < FN; ++i) {
+      f[q & 1][i] = fragment<BN>(gl + g_frag[i] + p * BM * BN + r * 16 * BN);
+    }
+  };
+  const auto multiply = [&](int q) {
+#pragma unroll
+    for (int i = 0; i < FN; ++i) {
+#pragma unroll
+      for (int j = 0; j < FK; ++j) {
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            f[q & 1][i], x[q / NP & 1][j], acc[i][j], 0, 0, 0);
       }
     }
-    // the next step's fragments are read before this step's products, which
-    // hide the read
-    bf16x8 f[2][FN], x[2][FK];
-    const auto read = [&](int q) {
-      const int r = q / NP, p = q % NP;
+  };
+  // the tiles of a row share the work of the bias's sum
+  const auto add_bias = [&](const short* gl, int stage) {
+    if (a.bias == nullptr || stage % a.tiles_k != tile.k) return;
 #pragma unroll
-      for (int j = 0; p == 0 && j < FK; ++j) {
-        x[r & 1][j] = fragment<BK>(xl + x_frag[j] + r * 16 * BK);
-      }
+    for (int i = 0; i < GC * NP; ++i) {
+      const int row = g_row + i % GC * kGDown;
+      float v[8];
+      load8(
+          (const __hip_bfloat16*)gl + i / GC * BM * BN +
+              slot<BN>(row, g_col / 8) * 8,
+          v);
 #pragma unroll
-      for (int i = 0; i < FN; ++i) {
-        f[q & 1][i] =
-            fragment<BN>(gl + g_frag[i] + p * BM * BN + r * 16 * BN);
-      }
-    };
-    read(0);
-#pragma unroll
-    for (int q = 0; q < kSteps * NP; ++q) {
-      if (q + 1 < kSteps * NP) read(q + 1);
-#pragma unroll
-      for (int i = 0; i < FN; ++i) {
-#pragma unroll
-        for (int j = 0; j < FK; ++j) {
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-              f[q & 1][i], x[q / NP & 1][j], acc[i][j], 0, 0, 0);
-        }
-      }
-      if (q % NP == NP - 1) other(q / NP);
+      for (int j = 0; j < 8; ++j) bias[j] += v[j];
     }
   };
 
@@ -269,26 +262,39 @@ __global__ __launch_bounds__(WN * WK * kWave) void wgrad8_kernel(WGrad a) {
       put_x(i, lds + NP * BM * BN);
       load_x(i, second);
     }
+    __syncthreads();
+    read(lds, 0);
   }
   for (int stage = 0; stage < fast; ++stage) {
-    __syncthreads();
+    const short* image = lds + (stage & 1) * kImage;
     short* next = lds + ((stage + 1) & 1) * kImage;
     // past the end the last stage is loaded again, and not used
     const int then = stage + 2 < fast ? stage + 2 : fast - 1;
-    products(lds + (stage & 1) * kImage, stage, [&](int r) {
-      // a share of the next stage goes to LDS while the products run, and
-      // its registers take the stage after that
+    add_bias(image, stage);
 #pragma unroll
-      for (int i = r * GC / kSteps; i < (r + 1) * GC / kSteps; ++i) {
+    for (int q = 0; q < kQ - 1; ++q) {
+      // Before the products of a step come the reads of the next one, behind
+      // them a share of the next stage, whose registers take the stage
+      // after that.
+      read(image, q + 1);
+      multiply(q);
+#pragma unroll
+      for (int i = q * GC / (kQ - 1); i < (q + 1) * GC / (kQ - 1); ++i) {
         put_g(i, next);
         load_g(i, then);
       }
 #pragma unroll
-      for (int i = r * XC / kSteps; i < (r + 1) * XC / kSteps; ++i) {
+      for (int i = q * XC / (kQ - 1); i < (q + 1) * XC / (kQ - 1); ++i) {
         put_x(i, next + NP * BM * BN);
         load_x(i, then);
       }
-    });
+    }
+    // The last step's fragments are in registers: the image is done with,
+    // and the next one whole behind the barrier, so that its first
+    // fragments are read before these products as well.
+    __syncthreads();
+    read(next, 0);
+    multiply(kQ - 1);
   }
   for (int stage = fast; stage < stages; ++stage) {
     // the end of the tokens: every value is checked
@@ -327,7 +333,12 @@ __global__ __launch_bounds__(WN * WK * kWave) void wgrad8_kernel(WGrad a) {
           lds + NP * BM * BN + slot<BK>(row, col / 8) * 8, h, 16);
     }
     __syncthreads();
-    products(lds, stage, [](int) {});
+    add_bias(lds, stage);
+#pragma unroll
+    for (int q = 0; q < kQ; ++q) {
+      read(lds, q);
+      multiply(q);
+    }
   }
 
   // column lane % 32, rows 8 * (r / 4) + 4 * (lane / 32) + r % 4
@@ -361,60 +372,157 @@ __global__ __launch_bounds__(WN * WK * kWave) void wgrad8_kernel(WGrad a) {
   }
 }
 
-// out[i] = sum over S of parts[s][i], 4 values a thread
+// One sum over rows: out[i] = sum over r < rows of parts[r][i], i < n.
+struct Sum {
+  const float* parts;
+  void* out;
+  long n;
+  int rows;
+  int type;
+};
+
+// Columns of a block: 4 a thread, with its 256 threads in `groups` that each
+// take every groups-th row.
+__host__ __device__ constexpr int sum_columns(int groups) {
+  return 1024 / groups;
+}
+constexpr int kWeightGroups = 4, kBiasGroups = 32;
+
+// Two sums in a launch, the weight's in the first `blocks` blocks, the
+// bias's behind them. The rows of a column are shared by 4 and by 32
+// threads: there are up to some 30 rows of the weight's sum, a few hundred
+// of the bias's, and a thread waits for each few that it reads.
 __global__ __launch_bounds__(256) void wgrad8_add_kernel(
-    const float* __restrict__ parts,
-    int S,
-    long n,
-    void* out,
-    int type) {
-  const long at = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (at >= n) return;
-  const int live = n - at < 4 ? (int)(n - at) : 4;
+    Sum weight,
+    unsigned blocks,
+    Sum bias) {
+  __shared__ float lds[1024];
+  const bool second = blockIdx.x >= blocks;
+  const Sum a = second ? bias : weight;
+  const int groups = second ? kBiasGroups : kWeightGroups;
+  const int lanes = 256 / groups;
+  const int group = threadIdx.x / lanes, lane = threadIdx.x % lanes;
+  const long first =
+      (long)(blockIdx.x - (second ? blocks : 0)) * sum_columns(groups);
+  const long at = first + lane * 4;
+  const int live = a.n - at < 4 ? (int)(a.n - at) : 4;
   float s[4] = {};
   if (live == 4) {
-#pragma unroll 4
-    for (int p = 0; p < S; ++p) {
+#pragma unroll 8
+    for (int r = group; r < a.rows; r += groups) {
       float v[4];
-      __builtin_memcpy(v, parts + p * n + at, 16);
+      __builtin_memcpy(v, a.parts + r * a.n + at, 16);
 #pragma unroll
       for (int j = 0; j < 4; ++j) s[j] += v[j];
     }
   } else {
-    for (int p = 0; p < S; ++p) {
-      for (int j = 0; j < live; ++j) s[j] += parts[p * n + at + j];
+#pragma unroll 4
+    for (int r = group; r < a.rows; r += groups) {
+#pragma unroll
+      for (int j = 0; j < 3; ++j) {
+        if (j < live) s[j] += a.parts[r * a.n + at + j];
+      }
     }
   }
-  for (int j = 0; j < live; ++j) store_any(out, type, at + j, s[j]);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) lds[group * lanes * 4 + lane * 4 + j] = s[j];
+  __syncthreads();
+  for (int c = threadIdx.x; c < lanes * 4; c += 256) {
+    if (first + c >= a.n) break;
+    float sum = 0.f;
+    for (int i = 0; i < groups; ++i) sum += lds[i * lanes * 4 + c];
+    store_any(a.out, a.type, first + c, sum);
+  }
 }
 
 }  // namespace
 
-// Tiles of 256 x 256 with 64 tokens a stage for bf16 gradients, 128 x 256
-// with 32 for those that are split: two images are 128 KB and 80 or 64 KB
-// of LDS.
+// bf16 numbers that a gradient is the sum of.
 template <typename TG>
+constexpr int kParts =
+    sizeof(TG) == 4 ? 3 : std::is_same<TG, __half>::value ? 2 : 1;
+
+// The tiles of a product, large and small. Two images are 128 KB of LDS for
+// large bf16 tiles, one block to a compute unit, and 80 KB or less for the
+// others, two blocks.
+template <typename TG, bool LARGE>
 struct Cut {
-  static constexpr int NP =
-      sizeof(TG) == 4 ? 3 : std::is_same<TG, __half>::value ? 2 : 1;
-  static constexpr int BN = NP == 1 ? 256 : 128, BK = 256;
+  static constexpr int NP = kParts<TG>;
+  static constexpr int BN = LARGE && NP == 1 ? 256 : 128;
+  static constexpr int BK = LARGE ? 256 : 128;
   static constexpr int BM = NP == 1 ? 64 : 32;
+  static constexpr int WN = 2, WK = LARGE ? 4 : 2;
+  static constexpr int kSlots = LARGE && NP == 1 ? 1 : 2;
+};
+
+// What a call takes, in us, by a model with the numbers of 40 shapes on
+// MI355X (rows 64 to 16384, widths 64 to 6144, each with some 20 splits;
+// the model is within 12 to 14 %, its choice 5 to 8 % from the best):
+// a block takes 8 to 10 us beside its stages, a stage the longer the fuller
+// the compute unit. Small tiles need more reads for each product (a stage
+// of a quarter of the area takes 1.2 us for two blocks, not 0.95), but
+// leave less to be added where the tokens are split.
+struct Rates {
+  float alone[2], full[2];  // a stage with half a card's blocks and with all
+  float block;
+  float add;       // a second launch
+  float per_byte;  // of the splits' sums, written and read
+  float per_row;   // of them
 };
 
 template <typename TG>
-WGradPlan wgrad8_plan(long M, int N, int K) {
-  using C = Cut<TG>;
-  WGradPlan p;
-  p.tiles_n = ceil_div(N, C::BN);
-  p.tiles_k = ceil_div(K, C::BK);
+constexpr Rates kRates = kParts<TG> == 1
+    ? Rates{{0.73f, 1.65f}, {1.22f, 1.89f}, 10.4f, 2.8f, 1.05e-7f, 0.06f}
+    : kParts<TG> == 2
+    ? Rates{{0.67f, 0.83f}, {1.00f, 2.14f}, 8.1f, 3.8f, 1.37e-7f, 0.06f}
+    : Rates{{0.91f, 1.17f}, {1.55f, 3.09f}, 8.6f, 3.2f, 1.36e-7f, 0.07f};
+
+template <typename TG, bool LARGE>
+void consider(long M, int N, int K, WGradPlan& best, float& best_time) {
+  using C = Cut<TG, LARGE>;
+  constexpr Rates rates = kRates<TG>;
+  constexpr int kSlots = 256 * C::kSlots;
+  const long tiles_n = ceil_div(N, C::BN), tiles_k = ceil_div(K, C::BK);
+  const long tiles = tiles_n * tiles_k;
   const long stages = (M + C::BM - 1) / C::BM;
-  const long tiles = (long)p.tiles_n * p.tiles_k;
-  long s = 256 / tiles;
-  if (s > stages / 4) s = stages / 4;
-  if (s < 1) s = 1;
-  p.rows = (stages + s - 1) / s * C::BM;
-  p.splits = (int)((M + p.rows - 1) / p.rows);
-  return p;
+  long last = 0;
+  for (const int blocks : {0, 64, 128, 192, 256, 384, 512}) {
+    long s = (blocks + tiles / 2) / tiles;
+    s = s < 1 ? 1 : s > stages ? stages : s;
+    const long per = (stages + s - 1) / s;
+    s = (stages + per - 1) / per;
+    if (s == last) continue;
+    last = s;
+    const long all = s * tiles, left = all % kSlots;
+    float time = (float)(all / kSlots) *
+        (rates.block + (float)per * rates.full[LARGE]);
+    if (left > 0) {
+      // from half a block for each compute unit to all of its blocks
+      float load = ((float)left / 256.f - 0.5f) / (C::kSlots - 0.5f);
+      load = load < 0.f ? 0.f : load;
+      time += rates.block +
+          (float)per *
+              (rates.alone[LARGE] +
+               load * (rates.full[LARGE] - rates.alone[LARGE]));
+    }
+    if (s > 1) {
+      time += rates.add + (float)s * rates.per_row +
+          (float)(s * N) * (float)K * 8.f * rates.per_byte;
+    }
+    if (time < best_time) {
+      best_time = time;
+      best = {LARGE, (int)s, (int)tiles_n, (int)tiles_k, per * C::BM};
+    }
+  }
+}
+
+template <typename TG>
+WGradPlan wgrad8_plan(long M, int N, int K) {
+  WGradPlan best{};
+  float time = __builtin_inff();
+  consider<TG, false>(M, N, K, best, time);
+  consider<TG, true>(M, N, K, best, time);
+  return best;
 }
 
 template <typename TG>
@@ -429,24 +537,40 @@ hipError_t wgrad8_t(
     const WGradPlan& plan,
     float* sums,
     float* bias) {
-  using C = Cut<TG>;
   WGrad a{g,    codes, exps, sums, bias, M, N, K, ceil_div(K, kBlock8),
           plan.tiles_n, plan.tiles_k, plan.rows};
   const unsigned grid = (unsigned)plan.splits * plan.tiles_n * plan.tiles_k;
-  wgrad8_kernel<TG, C::NP, C::BN, C::BK, C::BM, 2, 4>
-      <<<grid, 512, 0, s>>>(a);
-  return hipGetLastError();
+  const auto go = [&](auto large) {
+    using C = Cut<TG, decltype(large)::value>;
+    wgrad8_kernel<TG, C::NP, C::BN, C::BK, C::BM, C::WN, C::WK>
+        <<<grid, C::WN * C::WK * kWave, 0, s>>>(a);
+    return hipGetLastError();
+  };
+  return plan.large ? go(std::true_type()) : go(std::false_type());
 }
 
 hipError_t wgrad8_add(
     hipStream_t s,
-    const float* parts,
-    int S,
+    const float* sums,
+    int splits,
     long n,
     void* out,
+    const float* bias_sums,
+    int bias_rows,
+    long bias_n,
+    void* bias_out,
     int type) {
-  const long blocks = (n + 1023) / 1024;
-  wgrad8_add_kernel<<<(unsigned)blocks, 256, 0, s>>>(parts, S, n, out, type);
+  const Sum weight{sums, out, out == nullptr ? 0 : n, splits, type};
+  const Sum bias{
+      bias_sums, bias_out, bias_out == nullptr ? 0 : bias_n, bias_rows, type};
+  const auto blocks_of = [](long n, int groups) {
+    const int columns = sum_columns(groups);
+    return (unsigned)((n + columns - 1) / columns);
+  };
+  const unsigned blocks = blocks_of(weight.n, kWeightGroups);
+  const unsigned more = blocks_of(bias.n, kBiasGroups);
+  if (blocks + more == 0) return hipSuccess;
+  wgrad8_add_kernel<<<blocks + more, 256, 0, s>>>(weight, blocks, bias);
   return hipGetLastError();
 }
 
