@@ -237,6 +237,10 @@ struct Backward {
   const TX* dt;  // may be null
   TX* dx;
   float* partial;  // [gridDim.x][2][D], null if no parameter has a gradient
+                   // or a single block writes it
+  void* dw;        // either may be null
+  void* db;
+  int type;        // of both
   long R;
   int D;
   int blocks;
@@ -360,8 +364,18 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(Backward<TX, TY> a) {
       if (live && p.any) store8(lane_ptr(a.dx + start, p.col), d);
     }
   }
-  if (a.partial == nullptr) return;
-  float* mine = a.partial + (long)blockIdx.x * 2 * a.D;
+  // a single block's sums are the gradients
+  const bool single = a.partial == nullptr;
+  if (single && a.dw == nullptr && a.db == nullptr) return;
+  const auto put = [&](int which, int col, float v) {
+    if (!single) {
+      a.partial[((long)blockIdx.x * 2 + which) * a.D + col] = v;
+    } else if (which && a.db != nullptr) {
+      store_any(a.db, a.type, col, v);
+    } else if (!which && a.dw != nullptr) {
+      store_any(a.dw, a.type, col, v);
+    }
+  };
   if (G == 1) {
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
@@ -369,8 +383,8 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(Backward<TX, TY> a) {
 #pragma unroll
       for (int j = 0; j < kChunk; ++j) {
         if (p.any && j >= p.skip) {
-          mine[p.col + j] = dw[i][j];
-          mine[a.D + p.col + j] = db[i][j];
+          put(0, p.col + j, dw[i][j]);
+          put(1, p.col + j, db[i][j]);
         }
       }
     }
@@ -395,7 +409,7 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(Backward<TX, TY> a) {
       float s = 0.f;
 #pragma unroll
       for (int g = 0; g < G; ++g) s += parts[g * kSpan + c];
-      mine[which * a.D + c] = s;
+      put(which, c, s);
     }
   }
 }
@@ -407,9 +421,8 @@ __global__ __launch_bounds__(1024) void norm_param_kernel(
     int P,
     int D,
     void* dw,
-    int dw_type,
     void* db,
-    int db_type) {
+    int type) {
   __shared__ float lds[16][kWave];
   const int which = blockIdx.y;
   void* out = which ? db : dw;
@@ -430,7 +443,7 @@ __global__ __launch_bounds__(1024) void norm_param_kernel(
     s = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) s += lds[i][lane];
-    store_any(out, which ? db_type : dw_type, c, s);
+    store_any(out, type, c, s);
   }
 }
 
@@ -624,10 +637,17 @@ hipError_t by_width(int D, Fn fn) {
 
 }  // namespace
 
-int norm_bwd_partials(long R, int D) {
+// Blocks of the backward pass. Up to two rounds are left to a single block,
+// which then writes the gradients itself.
+static int norm_bwd_blocks(long R, int D) {
   if (is_long(D)) return (int)(R < kLongSplit ? R : kLongSplit);
   const long need = (R + rows_of_block(D) - 1) / rows_of_block(D);
-  return (int)(need < 256 ? need : 256);
+  return need <= 2 ? 1 : (int)(need < 256 ? need : 256);
+}
+
+int norm_bwd_partials(long R, int D) {
+  const int blocks = norm_bwd_blocks(R, D);
+  return blocks == 1 && !is_long(D) ? 0 : blocks;
 }
 
 template <typename TX, typename TY>
@@ -671,7 +691,6 @@ hipError_t norm_fwd_t(
   });
 }
 
-// partial: norm_bwd_partials(R, D) x 2 x D, or null (then dw and db too)
 template <typename TX, typename TY>
 hipError_t norm_bwd_t(
     hipStream_t s,
@@ -687,14 +706,14 @@ hipError_t norm_bwd_t(
     TX* dx,
     float* partial,
     void* dw,
-    int dw_type,
     void* db,
-    int db_type,
+    int type,
     long R,
     int D) {
-  Backward<TX, TY> a{dy, x,  codes,   exps, mean, rstd, {w, w_type},
-                     dt, dx, partial, R,    D,    ceil_div(D, kBlock8)};
-  const int P = norm_bwd_partials(R, D);
+  Backward<TX, TY> a{dy, x,       codes, exps, mean, rstd, {w, w_type}, dt,
+                     dx, partial, dw,    db,   type, R,    D,
+                     ceil_div(D, kBlock8)};
+  const int P = norm_bwd_blocks(R, D);
   if (is_long(D)) {
     norm_bwd_long_kernel<TX, TY><<<(unsigned)(R < 65536 ? R : 65536), 1024, 0, s>>>(a);
     KFAC_HIP_CHECK(hipGetLastError());
@@ -717,7 +736,7 @@ hipError_t norm_bwd_t(
   }
   if (partial == nullptr) return hipSuccess;
   norm_param_kernel<<<dim3(ceil_div(D, kWave), 2), 1024, 0, s>>>(
-      partial, P, D, dw, dw_type, db, db_type);
+      partial, P, D, dw, db, type);
   return hipGetLastError();
 }
 
@@ -729,7 +748,7 @@ hipError_t norm_bwd_t(
   template hipError_t norm_bwd_t<TX, TY>(                                     \
       hipStream_t, const TY*, const TX*, const int8_t*, const uint8_t*,       \
       const float*, const float*, const void*, int, const TX*, TX*, float*,   \
-      void*, int, void*, int, long, int);
+      void*, void*, int, long, int);
 KFAC_NORM(float, float)
 KFAC_NORM(float, __hip_bfloat16)
 KFAC_NORM(float, __half)

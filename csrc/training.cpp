@@ -1,11 +1,13 @@
 // Python binding of the transformer block's training kernels.
 //
-// Host-side glue only: checks that keep the kernels inside their tensors,
-// allocation, launches on the current stream of the tensors' device. All
-// tensors are contiguous here; the callers in kfac_amd.ops see to that.
+// Host-side glue only: the checks of the arguments (TypeError and ValueError
+// in Python, the same as kfac_amd.ops raises on the CPU), allocation,
+// launches on the current stream of the tensors' device. Small calls are
+// bound by the host, so allocation goes past the dispatcher.
 
 #include "training.h"
 
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
@@ -16,6 +18,7 @@ namespace {
 
 using torch::Tensor;
 using OptTensor = std::optional<Tensor>;
+using Borrowed = c10::MaybeOwned<Tensor>;
 
 #define CHECK_OK(expr)                                                       \
   do {                                                                       \
@@ -27,35 +30,40 @@ hipStream_t stream_of(const Tensor& t) {
   return c10::hip::getCurrentHIPStream(t.device().index()).stream();
 }
 
-void check(const Tensor& t, const char* name, const Tensor& like) {
-  TORCH_CHECK(t.is_cuda(), name, " must be a GPU tensor");
-  TORCH_CHECK(t.device() == like.device(), name, " is on another device");
-  TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+Tensor empty(
+    at::IntArrayRef size,
+    torch::ScalarType type,
+    const Tensor& like) {
+  return at::detail::empty_cuda(size, type, like.device(), std::nullopt);
+}
+
+Tensor zeros(
+    at::IntArrayRef size,
+    torch::ScalarType type,
+    const Tensor& like) {
+  return empty(size, type, like).zero_();
+}
+
+bool is_float(torch::ScalarType st) {
+  return st == torch::kFloat32 || st == torch::kBFloat16 ||
+      st == torch::kFloat16;
 }
 
 int type_of(torch::ScalarType st) {
-  switch (st) {
-    case torch::kFloat32:
-      return kfac::kF32;
-    case torch::kBFloat16:
-      return kfac::kBF16;
-    case torch::kFloat16:
-      return kfac::kF16;
-    default:
-      TORCH_CHECK(false, "unsupported dtype: ", st);
-  }
+  return st == torch::kFloat32 ? kfac::kF32
+      : st == torch::kBFloat16 ? kfac::kBF16
+                               : kfac::kF16;
 }
 
-// Calls fn with a value of the C++ type.
+// Calls fn with a value of the C++ type; the type has been checked.
 template <typename Fn>
 void by_type(torch::ScalarType st, Fn fn) {
-  switch (type_of(st)) {
-    case kfac::kF32:
-      return fn(float());
-    case kfac::kBF16:
-      return fn(__hip_bfloat16());
-    default:
-      return fn(__half());
+  if (st == torch::kFloat32) {
+    fn(float());
+  } else if (st == torch::kBFloat16) {
+    fn(__hip_bfloat16());
+  } else {
+    fn(__half());
   }
 }
 
@@ -65,19 +73,57 @@ struct Shape {
   long blocks;
 };
 
-Shape rows_of(const Tensor& t) {
-  TORCH_CHECK(t.dim() >= 1, "a tensor of rows has a dimension or more");
+Shape shape_of(const Tensor& t, const char* name) {
+  TORCH_CHECK_VALUE(
+      t.dim() >= 1 && t.size(-1) >= 1, name,
+      " must have rows of one value or more, got shape ", t.sizes());
   const long D = t.size(-1);
-  TORCH_CHECK(D > 0 && D < (1L << 30), "rows of 1 to 2^30 - 1 values");
+  TORCH_CHECK_VALUE(D < (1L << 30), name, " has rows of 2^30 values or more");
   return {t.numel() / D, (int)D, (D + kfac::kBlock8 - 1) / kfac::kBlock8};
 }
 
-// The two tensors of the 8 bit form of `like`.
+void check_float(torch::ScalarType st, const char* name) {
+  TORCH_CHECK_TYPE(
+      is_float(st), name, " must be float32, bfloat16 or float16, got ", st);
+}
+
+Shape check_rows(const Tensor& t, const char* name) {
+  check_float(t.scalar_type(), name);
+  TORCH_CHECK_VALUE(t.is_cuda(), name, " must be a GPU tensor");
+  return shape_of(t, name);
+}
+
+void check_like(const Tensor& t, const Tensor& like, const char* names) {
+  TORCH_CHECK_VALUE(
+      t.device() == like.device() && t.sizes() == like.sizes(), names,
+      " must have the same shape and device, got ", t.sizes(), " on ",
+      t.device(), " and ", like.sizes(), " on ", like.device());
+}
+
+Shape check_packed(const Tensor& codes, const Tensor& exps) {
+  TORCH_CHECK_TYPE(
+      codes.scalar_type() == torch::kInt8 &&
+          exps.scalar_type() == torch::kUInt8,
+      "a Packed8 holds int8 codes and uint8 exponents, got ",
+      codes.scalar_type(), " and ", exps.scalar_type());
+  TORCH_CHECK_VALUE(codes.is_cuda(), "codes must be a GPU tensor");
+  const Shape s = shape_of(codes, "codes");
+  TORCH_CHECK_VALUE(
+      exps.device() == codes.device() && exps.dim() == codes.dim() &&
+          exps.size(-1) == s.blocks &&
+          exps.sizes().slice(0, exps.dim() - 1) ==
+              codes.sizes().slice(0, codes.dim() - 1),
+      "codes of shape ", codes.sizes(), " do not go with exponents of shape ",
+      exps.sizes());
+  return s;
+}
+
+// The 8 bit form of a tensor like `like`: its codes, its exponents.
 std::tuple<Tensor, Tensor> empty_packed(const Tensor& like, long blocks) {
-  auto size = like.sizes().vec();
-  auto codes = torch::empty(size, like.options().dtype(torch::kInt8));
+  at::DimVector size(like.sizes());
+  auto codes = empty(size, torch::kInt8, like);
   size.back() = blocks;
-  return {codes, torch::empty(size, like.options().dtype(torch::kUInt8))};
+  return {std::move(codes), empty(size, torch::kUInt8, like)};
 }
 
 // The 8 bit forms of an input and an output that a call asks for, null where
@@ -97,52 +143,44 @@ struct Packs {
       auto [c, e] = empty_packed(like, blocks);
       codes[i] = (int8_t*)c.data_ptr();
       exps[i] = (uint8_t*)e.data_ptr();
-      out.push_back(c);
-      out.push_back(e);
+      out.push_back(std::move(c));
+      out.push_back(std::move(e));
     }
   }
 };
 
-Shape check_packed(
-    const Tensor& codes,
-    const Tensor& exps,
-    const Tensor& like) {
-  check(codes, "codes", like);
-  check(exps, "exponents", like);
-  TORCH_CHECK(codes.scalar_type() == torch::kInt8, "codes must be int8");
-  TORCH_CHECK(exps.scalar_type() == torch::kUInt8, "exponents must be uint8");
-  const Shape s = rows_of(codes);
-  TORCH_CHECK(
-      exps.numel() == s.R * s.blocks, "codes and exponents do not match");
-  return s;
-}
-
-std::tuple<Tensor, Tensor> pack8(Tensor x) {
-  check(x, "x", x);
+std::tuple<Tensor, Tensor> pack8(const Tensor& x) {
+  const Shape s = check_rows(x, "x");
   const c10::DeviceGuard guard(x.device());
-  const Shape s = rows_of(x);
-  auto [codes, exps] = empty_packed(x, s.blocks);
+  const Borrowed xc = x.expect_contiguous();
+  auto packed = empty_packed(x, s.blocks);
   if (s.R > 0) {
     by_type(x.scalar_type(), [&](auto t) {
       using T = decltype(t);
       CHECK_OK(kfac::pack8_t<T>(
-          stream_of(x), (const T*)x.const_data_ptr(),
-          (int8_t*)codes.data_ptr(), (uint8_t*)exps.data_ptr(), s.R, s.D));
+          stream_of(x), (const T*)xc->const_data_ptr(),
+          (int8_t*)std::get<0>(packed).data_ptr(),
+          (uint8_t*)std::get<1>(packed).data_ptr(), s.R, s.D));
     });
   }
-  return {codes, exps};
+  return packed;
 }
 
-Tensor unpack8(Tensor codes, Tensor exps, torch::ScalarType dtype) {
-  const Shape s = check_packed(codes, exps, codes);
+Tensor unpack8(
+    const Tensor& codes,
+    const Tensor& exps,
+    torch::ScalarType dtype) {
+  const Shape s = check_packed(codes, exps);
+  check_float(dtype, "dtype");
   const c10::DeviceGuard guard(codes.device());
-  auto out = torch::empty(codes.sizes(), codes.options().dtype(dtype));
+  const Borrowed cc = codes.expect_contiguous(), ec = exps.expect_contiguous();
+  auto out = empty(codes.sizes(), dtype, codes);
   if (s.R > 0) {
     by_type(dtype, [&](auto t) {
       using T = decltype(t);
       CHECK_OK(kfac::unpack8_t<T>(
-          stream_of(codes), (const int8_t*)codes.const_data_ptr(),
-          (const uint8_t*)exps.const_data_ptr(), (T*)out.data_ptr(), s.R,
+          stream_of(codes), (const int8_t*)cc->const_data_ptr(),
+          (const uint8_t*)ec->const_data_ptr(), (T*)out.data_ptr(), s.R,
           s.D));
     });
   }
@@ -151,243 +189,278 @@ Tensor unpack8(Tensor codes, Tensor exps, torch::ScalarType dtype) {
 
 // (y[, codes and exponents of x][, of y])
 std::vector<Tensor> gelu8_forward(
-    Tensor x,
+    const Tensor& x,
     bool tanh,
     bool pack_input,
     bool pack_output) {
-  check(x, "x", x);
+  const Shape s = check_rows(x, "x");
   const c10::DeviceGuard guard(x.device());
-  const Shape s = rows_of(x);
-  auto y = torch::empty_like(x);
-  std::vector<Tensor> out{y};
+  const Borrowed xc = x.expect_contiguous();
+  std::vector<Tensor> out{empty(x.sizes(), x.scalar_type(), x)};
   const Packs packs(x, s.blocks, pack_input, pack_output, out);
   if (s.R > 0) {
     by_type(x.scalar_type(), [&](auto t) {
       using T = decltype(t);
       CHECK_OK(kfac::gelu8_fwd_t<T>(
-          stream_of(x), (const T*)x.const_data_ptr(), (T*)y.data_ptr(),
-          packs.codes[0], packs.exps[0], packs.codes[1], packs.exps[1], s.R,
-          s.D, tanh));
+          stream_of(x), (const T*)xc->const_data_ptr(),
+          (T*)out[0].data_ptr(), packs.codes[0], packs.exps[0],
+          packs.codes[1], packs.exps[1], s.R, s.D, tanh));
     });
   }
   return out;
 }
 
-Tensor gelu8_backward(Tensor dy, Tensor codes, Tensor exps, bool tanh) {
-  check(dy, "dy", dy);
-  const Shape s = check_packed(codes, exps, dy);
-  TORCH_CHECK(dy.sizes() == codes.sizes(), "dy and the input do not match");
+Tensor gelu8_backward(
+    const Tensor& dy,
+    const Tensor& codes,
+    const Tensor& exps,
+    bool tanh) {
+  check_rows(dy, "dy");
+  const Shape s = check_packed(codes, exps);
+  check_like(dy, codes, "dy and the packed input");
   const c10::DeviceGuard guard(dy.device());
-  auto dx = torch::empty_like(dy);
+  const Borrowed dc = dy.expect_contiguous();
+  const Borrowed cc = codes.expect_contiguous(), ec = exps.expect_contiguous();
+  auto dx = empty(dy.sizes(), dy.scalar_type(), dy);
   if (s.R > 0) {
     by_type(dy.scalar_type(), [&](auto t) {
       using T = decltype(t);
       CHECK_OK(kfac::gelu8_bwd_t<T>(
-          stream_of(dy), (const T*)dy.const_data_ptr(),
-          (const int8_t*)codes.const_data_ptr(),
-          (const uint8_t*)exps.const_data_ptr(), (T*)dx.data_ptr(), s.R, s.D,
+          stream_of(dy), (const T*)dc->const_data_ptr(),
+          (const int8_t*)cc->const_data_ptr(),
+          (const uint8_t*)ec->const_data_ptr(), (T*)dx.data_ptr(), s.R, s.D,
           tanh));
     });
   }
   return dx;
 }
 
-// Calls fn with values of both types: the same, or one of them fp32.
+// The types of a norm's inner (x, dx) and outer (y, dy) tensors: the same,
+// or one of them fp32.
+void check_types(torch::ScalarType inner, torch::ScalarType outer) {
+  TORCH_CHECK_TYPE(
+      is_float(outer) &&
+          (inner == outer || inner == torch::kFloat32 ||
+           outer == torch::kFloat32),
+      "no layer norm from ", inner, " to ", outer,
+      ": the types must be the same or one of them float32");
+}
+
 template <typename Fn>
 void by_types(torch::ScalarType x, torch::ScalarType y, Fn fn) {
   by_type(x, [&](auto tx) {
     using TX = decltype(tx);
     if (x == y) {
       fn(tx, tx);
-    } else if (y == torch::kFloat32) {
-      fn(tx, float());
     } else if constexpr (std::is_same_v<TX, float>) {
       by_type(y, [&](auto ty) { fn(tx, ty); });
     } else {
-      TORCH_CHECK(false, "no layer norm between ", x, " and ", y);
+      fn(tx, float());
     }
   });
 }
 
-const void* ptr_or_null(const OptTensor& t) {
-  return t ? t->const_data_ptr() : nullptr;
-}
-int type_or_f32(const OptTensor& t) {
-  return t ? type_of(t->scalar_type()) : kfac::kF32;
-}
+// A tensor that may be missing: contiguous, with its pointer and type.
+struct Param {
+  std::optional<Borrowed> held;
+  const void* p = nullptr;
+  int type = kfac::kF32;
+
+  explicit Param(const OptTensor& t) {
+    if (!t) return;
+    held.emplace(t->expect_contiguous());
+    p = (*held)->const_data_ptr();
+    if (is_float(t->scalar_type())) type = type_of(t->scalar_type());
+  }
+};
 
 void check_param(const OptTensor& t, const char* name, const Tensor& x) {
   if (!t) return;
-  check(*t, name, x);
-  TORCH_CHECK(t->numel() == x.size(-1), name, " does not fit the rows");
+  check_float(t->scalar_type(), name);
+  TORCH_CHECK_VALUE(
+      t->dim() == 1 && t->size(0) == x.size(-1) && t->device() == x.device(),
+      name, " must have shape (", x.size(-1), ",) on ", x.device(), ", got ",
+      t->sizes(), " on ", t->device());
 }
 
 // (y, total or x, mean, rstd[, codes, exponents of the input][, of the
 // output])
 std::vector<Tensor> norm_forward(
-    Tensor x,
-    OptTensor r,
-    OptTensor w,
-    OptTensor b,
+    const Tensor& x,
+    const OptTensor& r,
+    const OptTensor& w,
+    const OptTensor& b,
     double eps,
-    torch::ScalarType dtype,
+    std::optional<torch::ScalarType> out_dtype,
     bool pack_input,
     bool pack_output) {
-  check(x, "x", x);
-  const c10::DeviceGuard guard(x.device());
-  const Shape s = rows_of(x);
+  const Shape s = check_rows(x, "x");
+  const auto xt = x.scalar_type(), yt = out_dtype.value_or(xt);
+  check_types(xt, yt);
   check_param(w, "weight", x);
   check_param(b, "bias", x);
   if (r) {
-    check(*r, "residual", x);
-    TORCH_CHECK(r->sizes() == x.sizes(), "x and residual do not match");
+    check_float(r->scalar_type(), "residual");
+    check_like(x, *r, "x and residual");
+    TORCH_CHECK_TYPE(
+        r->scalar_type() == xt || xt == torch::kFloat32, "a residual of ",
+        r->scalar_type(), " does not fit a sum of ", xt);
   }
-  auto y = torch::empty(x.sizes(), x.options().dtype(dtype));
-  auto total = r ? torch::empty_like(x) : x;
-  auto mean = torch::empty({s.R}, x.options().dtype(torch::kFloat32));
-  auto rstd = torch::empty_like(mean);
-  std::vector<Tensor> out{y, total, mean, rstd};
+  const c10::DeviceGuard guard(x.device());
+  const Borrowed xc = x.expect_contiguous();
+  const Param rp(r), wp(w), bp(b);
+  std::vector<Tensor> out;
+  out.reserve(8);
+  out.push_back(empty(x.sizes(), yt, x));
+  out.push_back(r ? empty(x.sizes(), xt, x) : *xc);
+  out.push_back(empty({s.R}, torch::kFloat32, x));
+  out.push_back(empty({s.R}, torch::kFloat32, x));
   const Packs packs(x, s.blocks, pack_input, pack_output, out);
   if (s.R > 0) {
-    by_types(x.scalar_type(), dtype, [&](auto tx, auto ty) {
+    by_types(xt, yt, [&](auto tx, auto ty) {
       using TX = decltype(tx);
       using TY = decltype(ty);
       CHECK_OK((kfac::norm_fwd_t<TX, TY>(
-          stream_of(x), (const TX*)x.const_data_ptr(), ptr_or_null(r),
-          type_or_f32(r), ptr_or_null(w), type_or_f32(w), ptr_or_null(b),
-          type_or_f32(b), r ? (TX*)total.data_ptr() : nullptr,
-          (TY*)y.data_ptr(), mean.data_ptr<float>(), rstd.data_ptr<float>(),
-          packs.codes[0], packs.exps[0], packs.codes[1], packs.exps[1], s.R,
-          s.D, (float)eps)));
+          stream_of(x), (const TX*)xc->const_data_ptr(), rp.p, rp.type, wp.p,
+          wp.type, bp.p, bp.type, r ? (TX*)out[1].data_ptr() : nullptr,
+          (TY*)out[0].data_ptr(), (float*)out[2].data_ptr(),
+          (float*)out[3].data_ptr(), packs.codes[0], packs.exps[0],
+          packs.codes[1], packs.exps[1], s.R, s.D, (float)eps)));
     });
   }
   return out;
 }
 
-// (dx, dweight or None, dbias or None); x or (codes, exps)
+// (dx, dweight or None, dbias or None); total or (codes, exps)
 std::tuple<Tensor, OptTensor, OptTensor> norm_backward(
-    Tensor dy,
-    OptTensor x,
-    OptTensor codes,
-    OptTensor exps,
-    Tensor mean,
-    Tensor rstd,
-    OptTensor w,
-    bool want_dw,
+    const Tensor& dy,
+    const OptTensor& total,
+    const OptTensor& codes,
+    const OptTensor& exps,
+    const Tensor& mean,
+    const Tensor& rstd,
+    const OptTensor& w,
     bool want_db,
-    OptTensor dt,
-    torch::ScalarType dtype) {
-  check(dy, "dy", dy);
-  const c10::DeviceGuard guard(dy.device());
-  const Shape s = rows_of(dy);
-  if (x) {
-    check(*x, "x", dy);
-    TORCH_CHECK(
-        x->sizes() == dy.sizes() && x->scalar_type() == dtype,
-        "x and dy do not match");
+    const OptTensor& dt,
+    std::optional<torch::ScalarType> dtype) {
+  const Shape s = check_rows(dy, "dy");
+  auto xt = dy.scalar_type();
+  if (total) {
+    check_float(total->scalar_type(), "total");
+    check_like(dy, *total, "dy and total");
+    xt = total->scalar_type();
+    TORCH_CHECK_TYPE(
+        !dtype || *dtype == xt, "dx has the type of total, ", xt);
   } else {
-    TORCH_CHECK(codes && exps, "x or its 8 bit form");
-    check_packed(*codes, *exps, dy);
-    TORCH_CHECK(codes->sizes() == dy.sizes(), "x and dy do not match");
+    TORCH_CHECK_VALUE(codes && exps, "total or its 8 bit form is missing");
+    check_packed(*codes, *exps);
+    check_like(dy, *codes, "dy and total");
+    xt = dtype.value_or(xt);
+    check_float(xt, "dtype");
   }
-  check(mean, "mean", dy);
-  check(rstd, "rstd", dy);
-  TORCH_CHECK(
-      mean.scalar_type() == torch::kFloat32 &&
-          rstd.scalar_type() == torch::kFloat32 && mean.numel() == s.R &&
-          rstd.numel() == s.R,
-      "mean and rstd must be fp32, one a row");
+  check_types(xt, dy.scalar_type());
   check_param(w, "weight", dy);
+  for (const auto* t : {&mean, &rstd}) {
+    TORCH_CHECK_VALUE(
+        t->scalar_type() == torch::kFloat32 && t->dim() == 1 &&
+            t->size(0) == s.R && t->device() == dy.device(),
+        t == &mean ? "mean" : "rstd", " must hold a float32 for each row");
+  }
   if (dt) {
-    check(*dt, "grad_total", dy);
-    TORCH_CHECK(
-        dt->sizes() == dy.sizes() && dt->scalar_type() == dtype,
-        "grad_total and dx do not match");
+    check_like(dy, *dt, "dy and grad_total");
+    TORCH_CHECK_TYPE(
+        dt->scalar_type() == xt, "grad_total must be ", xt, ", as dx is");
   }
-  auto dx = torch::empty(dy.sizes(), dy.options().dtype(dtype));
-  const auto ptype = w ? w->scalar_type() : torch::kFloat32;
-  const auto popts = dy.options().dtype(ptype);
+  const c10::DeviceGuard guard(dy.device());
+  const Borrowed dc = dy.expect_contiguous();
+  const Borrowed mc = mean.expect_contiguous(), rc = rstd.expect_contiguous();
+  const Param xp(total), cp(codes), ep(exps), wp(w), tp(dt);
+  auto dx = empty(dy.sizes(), xt, dy);
+  const auto pt = w ? w->scalar_type() : torch::kFloat32;
   OptTensor dw, db;
-  const std::vector<int64_t> size{s.D};
-  if (want_dw) dw = s.R ? torch::empty(size, popts) : torch::zeros(size, popts);
-  if (want_db) db = s.R ? torch::empty(size, popts) : torch::zeros(size, popts);
-  if (s.R == 0) return {dx, dw, db};
-  Tensor partial;
-  if (want_dw || want_db) {
-    partial = torch::empty(
-        {(long)kfac::norm_bwd_partials(s.R, s.D) * 2 * s.D},
-        dy.options().dtype(torch::kFloat32));
+  if (s.R == 0) {
+    if (w) dw = zeros({s.D}, pt, dy);
+    if (want_db) db = zeros({s.D}, pt, dy);
+    return {dx, dw, db};
   }
-  by_types(dtype, dy.scalar_type(), [&](auto tx, auto ty) {
+  if (w) dw = empty({s.D}, pt, dy);
+  if (want_db) db = empty({s.D}, pt, dy);
+  Tensor partial;
+  const long rows = dw || db ? kfac::norm_bwd_partials(s.R, s.D) : 0;
+  if (rows > 0) partial = empty({rows * 2 * s.D}, torch::kFloat32, dy);
+  by_types(xt, dy.scalar_type(), [&](auto tx, auto ty) {
     using TX = decltype(tx);
     using TY = decltype(ty);
     CHECK_OK((kfac::norm_bwd_t<TX, TY>(
-        stream_of(dy), (const TY*)dy.const_data_ptr(),
-        (const TX*)ptr_or_null(x), (const int8_t*)ptr_or_null(codes),
-        (const uint8_t*)ptr_or_null(exps), mean.data_ptr<float>(),
-        rstd.data_ptr<float>(), ptr_or_null(w), type_or_f32(w),
-        (const TX*)ptr_or_null(dt), (TX*)dx.data_ptr(),
-        partial.defined() ? partial.data_ptr<float>() : nullptr,
-        dw ? dw->data_ptr() : nullptr, type_of(ptype),
-        db ? db->data_ptr() : nullptr, type_of(ptype), s.R, s.D)));
+        stream_of(dy), (const TY*)dc->const_data_ptr(), (const TX*)xp.p,
+        (const int8_t*)cp.p, (const uint8_t*)ep.p,
+        (const float*)mc->const_data_ptr(),
+        (const float*)rc->const_data_ptr(), wp.p, wp.type, (const TX*)tp.p,
+        (TX*)dx.data_ptr(),
+        partial.defined() ? (float*)partial.data_ptr() : nullptr,
+        dw ? dw->data_ptr() : nullptr, db ? db->data_ptr() : nullptr,
+        type_of(pt), s.R, s.D)));
   });
-  return {dx, dw, db};
+  return {std::move(dx), std::move(dw), std::move(db)};
 }
 
 // (dW, db or None)
 std::tuple<Tensor, OptTensor> weight_grad8(
-    Tensor g,
-    Tensor codes,
-    Tensor exps,
+    const Tensor& g,
+    const Tensor& codes,
+    const Tensor& exps,
     bool want_bias,
     torch::ScalarType dtype) {
-  check(g, "g", g);
+  const Shape sg = check_rows(g, "g");
+  const Shape sx = check_packed(codes, exps);
+  TORCH_CHECK_VALUE(
+      g.device() == codes.device() && g.dim() == codes.dim() &&
+          g.sizes().slice(0, g.dim() - 1) ==
+              codes.sizes().slice(0, codes.dim() - 1),
+      "g and the packed input must have the same rows and device, got ",
+      g.sizes(), " on ", g.device(), " and ", codes.sizes(), " on ",
+      codes.device());
+  check_float(dtype, "dtype");
   const c10::DeviceGuard guard(g.device());
-  const Shape sx = check_packed(codes, exps, g);
-  const Shape sg = rows_of(g);
-  TORCH_CHECK(sx.R == sg.R, "the gradient and the input have other rows");
-  const long M = sg.R;
-  const long N = sg.D, K = sx.D;
-  const auto opts = g.options().dtype(dtype);
-  const auto f32 = g.options().dtype(torch::kFloat32);
-  const std::vector<int64_t> size{N, K}, bias_size{N};
+  const Borrowed gc = g.expect_contiguous();
+  const Borrowed cc = codes.expect_contiguous(), ec = exps.expect_contiguous();
+  const long M = sg.R, N = sg.D, K = sx.D;
   OptTensor db;
   if (M == 0) {
-    if (want_bias) db = torch::zeros(bias_size, opts);
-    return {torch::zeros(size, opts), db};
+    if (want_bias) db = zeros({N}, dtype, g);
+    return {zeros({N, K}, dtype, g), db};
   }
-  kfac::WGradPlan plan;
-  by_type(g.scalar_type(), [&](auto t) {
-    plan = kfac::wgrad8_plan<decltype(t)>(M, sg.D, sx.D);
-  });
-  const long rows = (long)plan.splits * plan.tiles_k;
-  auto dw = torch::empty(size, opts);
-  if (want_bias) db = torch::empty(bias_size, opts);
-  // a single fp32 sum is the result itself
-  const bool direct = plan.splits == 1 && dtype == torch::kFloat32;
-  const bool bias_direct = rows == 1 && dtype == torch::kFloat32;
-  Tensor sums = dw, bias = want_bias ? *db : Tensor();
-  if (!direct) {
-    sums = torch::empty({plan.splits * N * K}, f32);
-  }
-  if (want_bias && !bias_direct) bias = torch::empty({rows * N}, f32);
+  auto dw = empty({N, K}, dtype, g);
+  if (want_bias) db = empty({N}, dtype, g);
   const auto stream = stream_of(g);
   by_type(g.scalar_type(), [&](auto t) {
     using T = decltype(t);
+    const auto plan = kfac::wgrad8_plan<T>(M, sg.D, sx.D);
+    const long rows = (long)plan.splits * plan.tiles_k;
+    // a single fp32 sum is the result itself; the others share a workspace
+    const bool direct = plan.splits == 1 && dtype == torch::kFloat32;
+    const bool bias_direct = rows == 1 && dtype == torch::kFloat32;
+    const long need = direct ? 0 : plan.splits * N * K;
+    const long bias_need = want_bias && !bias_direct ? rows * N : 0;
+    Tensor work;
+    float* sums = (float*)dw.data_ptr();
+    float* bias = want_bias ? (float*)db->data_ptr() : nullptr;
+    if (need + bias_need > 0) {
+      work = empty({need + bias_need}, torch::kFloat32, g);
+      if (need > 0) sums = (float*)work.data_ptr();
+      if (bias_need > 0) bias = (float*)work.data_ptr() + need;
+    }
     CHECK_OK(kfac::wgrad8_t<T>(
-        stream, (const T*)g.const_data_ptr(),
-        (const int8_t*)codes.const_data_ptr(),
-        (const uint8_t*)exps.const_data_ptr(), M, sg.D, sx.D, plan,
-        sums.data_ptr<float>(),
-        want_bias ? bias.data_ptr<float>() : nullptr));
+        stream, (const T*)gc->const_data_ptr(),
+        (const int8_t*)cc->const_data_ptr(),
+        (const uint8_t*)ec->const_data_ptr(), M, sg.D, sx.D, plan, sums,
+        bias));
+    CHECK_OK(kfac::wgrad8_add(
+        stream, sums, plan.splits, N * K, need ? dw.data_ptr() : nullptr,
+        bias, (int)rows, N, bias_need ? db->data_ptr() : nullptr,
+        type_of(dtype)));
   });
-  const bool add_bias = want_bias && !bias_direct;
-  CHECK_OK(kfac::wgrad8_add(
-      stream, sums.data_ptr<float>(), plan.splits, N * K,
-      direct ? nullptr : dw.data_ptr(),
-      add_bias ? bias.data_ptr<float>() : nullptr, (int)rows, N,
-      add_bias ? db->data_ptr() : nullptr, type_of(dtype)));
-  return {dw, db};
+  return {std::move(dw), std::move(db)};
 }
 
 }  // namespace

@@ -40,16 +40,18 @@ hipError_t norm_fwd_t(
     int w_type, const void* b, int b_type, TX* total, TY* y, float* mean,
     float* rstd, int8_t* in_codes, uint8_t* in_exps, int8_t* out_codes,
     uint8_t* out_exps, long R, int D, float eps);
-// rows of the workspace that the backward pass sums parameters in
+// rows of the workspace that the backward pass sums the parameters'
+// gradients in, which may be 0
 int norm_bwd_partials(long R, int D);
 // x or (codes, exps); w, dt, dw, db may be null. partial holds
-// norm_bwd_partials(R, D) x 2 x D floats, or is null if dw and db are.
+// norm_bwd_partials(R, D) x 2 x D floats, or is null if that is 0 or there
+// is neither dw nor db.
 template <typename TX, typename TY>
 hipError_t norm_bwd_t(
     hipStream_t, const TY* dy, const TX* x, const int8_t* codes,
     const uint8_t* exps, const float* mean, const float* rstd, const void* w,
-    int w_type, const TX* dt, TX* dx, float* partial, void* dw, int dw_type,
-    void* db, int db_type, long R, int D);
+    int w_type, const TX* dt, TX* dx, float* partial, void* dw, void* db,
+    int type, long R, int D);
 
 // How a weight gradient is cut into blocks.
 struct WGradPlan {

@@ -50,6 +50,9 @@ class Activated8(NamedTuple):
     packed_output: Packed8 | None
 
 
+# The checks below are those of the CPU; csrc/training.cpp has the same.
+
+
 def check_rows(x: torch.Tensor, name: str) -> None:
     """Raise unless ``x`` is a tensor of rows of one or more floats."""
     if x.dtype not in FLOAT_TYPES:
@@ -115,11 +118,11 @@ def pack8(x: torch.Tensor) -> Packed8:
     off by at most 2^(e-1); zero stays zero. ``x`` may be float32, bfloat16
     or float16, of any strides.
     """
-    check_rows(x, 'x')
     if x.is_cuda:
         ext = ops._require_ext('pack8')
         if ext is not None:
-            return Packed8(*ext.pack8(x.contiguous()))
+            return Packed8(*ext.pack8(x))
+    check_rows(x, 'x')
     return Packed8(*ref.pack8(x))
 
 
@@ -132,14 +135,14 @@ def unpack8(
     Exact in float32 and bfloat16 (a code times a power of two has 7 bits);
     rounded, and beyond 65504 infinite, in float16.
     """
-    check_packed(packed)
-    if dtype not in FLOAT_TYPES:
-        raise TypeError(f'no values of type {dtype}')
     codes, exps = packed
     if codes.is_cuda:
         ext = ops._require_ext('unpack8')
         if ext is not None:
-            return ext.unpack8(codes.contiguous(), exps.contiguous(), dtype)
+            return ext.unpack8(codes, exps, dtype)
+    check_packed(packed)
+    if dtype not in FLOAT_TYPES:
+        raise TypeError(f'no values of type {dtype}')
     return ref.unpack8(codes, exps, dtype)
 
 
@@ -157,22 +160,19 @@ def gelu8_forward(
     as ``pack8(y)``, without reading y again. ``packed_input=False`` leaves
     out what only a backward pass needs.
     """
-    check_rows(x, 'x')
     check_approximate(approximate)
     if x.is_cuda:
         ext = ops._require_ext('gelu8_forward')
         if ext is not None:
             y, *packed = ext.gelu8_forward(
-                x.contiguous(),
-                approximate == 'tanh',
-                packed_input,
-                packed_output,
+                x, approximate == 'tanh', packed_input, packed_output,
             )
             return Activated8(
                 y,
                 Packed8(*packed[:2]) if packed_input else None,
                 Packed8(*packed[-2:]) if packed_output else None,
             )
+    check_rows(x, 'x')
     y = ref.gelu(x, approximate)
     return Activated8(
         y,
@@ -188,20 +188,15 @@ def gelu8_backward(
     approximate: str = 'none',
 ) -> torch.Tensor:
     """Gradient of GELU's input, whose 8 bit form was kept; in dy's type."""
-    check_rows(dy, 'dy')
-    check_packed(packed_input)
     check_approximate(approximate)
     codes, exps = packed_input
-    check_same_shape(dy, codes, 'dy and the packed input')
     if dy.is_cuda:
         ext = ops._require_ext('gelu8_backward')
         if ext is not None:
-            return ext.gelu8_backward(
-                dy.contiguous(),
-                codes.contiguous(),
-                exps.contiguous(),
-                approximate == 'tanh',
-            )
+            return ext.gelu8_backward(dy, codes, exps, approximate == 'tanh')
+    check_rows(dy, 'dy')
+    check_packed(packed_input)
+    check_same_shape(dy, codes, 'dy and the packed input')
     return ref.gelu_backward(dy, ref.unpack8(codes, exps), approximate)
 
 
@@ -221,9 +216,13 @@ def weight_grad8(
     are rounded once to ``dtype``. Without rows they are zero. The same
     inputs give the same bits each time.
     """
+    codes, exps = packed_input
+    if g.is_cuda:
+        ext = ops._require_ext('weight_grad8')
+        if ext is not None:
+            return ext.weight_grad8(g, codes, exps, bias, dtype)
     check_rows(g, 'g')
     check_packed(packed_input)
-    codes, exps = packed_input
     if g.shape[:-1] != codes.shape[:-1] or g.device != codes.device:
         raise ValueError(
             'g and the packed input must have the same rows and device, got '
@@ -232,16 +231,6 @@ def weight_grad8(
         )
     if dtype not in FLOAT_TYPES:
         raise TypeError(f'no gradients of type {dtype}')
-    if g.is_cuda:
-        ext = ops._require_ext('weight_grad8')
-        if ext is not None:
-            return ext.weight_grad8(
-                g.contiguous(),
-                codes.contiguous(),
-                exps.contiguous(),
-                bias,
-                dtype,
-            )
     return ref.weight_grad(g, ref.unpack8(codes, exps), bias, dtype)
 
 

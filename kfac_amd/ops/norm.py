@@ -44,7 +44,7 @@ class Normed(NamedTuple):
 
 
 def _check_types(inner: torch.dtype, outer: torch.dtype) -> None:
-    if outer not in FLOAT_TYPES or (
+    if inner not in FLOAT_TYPES or outer not in FLOAT_TYPES or (
         inner != outer and torch.float32 not in (inner, outer)
     ):
         raise TypeError(
@@ -91,27 +91,14 @@ def layer_norm_forward(
             :func:`layer_norm_backward` takes in its place.
         packed_output: return the 8 bit form of y, the same as ``pack8(y)``.
     """
-    check_rows(x, 'x')
-    out_dtype = x.dtype if out_dtype is None else out_dtype
-    _check_types(x.dtype, out_dtype)
-    _check_param(weight, 'weight', x)
-    _check_param(bias, 'bias', x)
-    if residual is not None:
-        check_rows(residual, 'residual')
-        check_same_shape(x, residual, 'x and residual')
-        if torch.promote_types(x.dtype, residual.dtype) != x.dtype:
-            raise TypeError(
-                f'a residual of {residual.dtype} does not fit a sum of '
-                f'{x.dtype}',
-            )
     if x.is_cuda:
         ext = ops._require_ext('layer_norm_forward')
         if ext is not None:
             y, total, mean, rstd, *packed = ext.norm_forward(
-                x.contiguous(),
-                None if residual is None else residual.contiguous(),
-                None if weight is None else weight.contiguous(),
-                None if bias is None else bias.contiguous(),
+                x,
+                residual,
+                weight,
+                bias,
                 eps,
                 out_dtype,
                 packed_input,
@@ -124,6 +111,19 @@ def layer_norm_forward(
                 rstd,
                 Packed8(*packed[:2]) if packed_input else None,
                 Packed8(*packed[-2:]) if packed_output else None,
+            )
+    check_rows(x, 'x')
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    _check_types(x.dtype, out_dtype)
+    _check_param(weight, 'weight', x)
+    _check_param(bias, 'bias', x)
+    if residual is not None:
+        check_rows(residual, 'residual')
+        check_same_shape(x, residual, 'x and residual')
+        if torch.promote_types(x.dtype, residual.dtype) != x.dtype:
+            raise TypeError(
+                f'a residual of {residual.dtype} does not fit a sum of '
+                f'{x.dtype}',
             )
     y, total, mean, rstd = ref.layer_norm_forward(
         x, weight, bias, eps, residual, out_dtype,
@@ -165,18 +165,34 @@ def layer_norm_backward(
     The parameters' gradients come in the weight's type (float32 without a
     weight). The same inputs give the same bits each time.
     """
+    packed = not isinstance(total, torch.Tensor)
+    if dy.is_cuda:
+        ext = ops._require_ext('layer_norm_backward')
+        if ext is not None:
+            return ext.norm_backward(
+                dy,
+                None if packed else total,
+                total[0] if packed else None,
+                total[1] if packed else None,
+                mean,
+                rstd,
+                weight,
+                bias,
+                grad_total,
+                dtype,
+            )
     check_rows(dy, 'dy')
-    if isinstance(total, torch.Tensor):
+    if packed:
+        check_packed(total)
+        check_same_shape(dy, total.codes, 'dy and total')
+        dtype = dy.dtype if dtype is None else dtype
+    else:
         check_rows(total, 'total')
         check_same_shape(dy, total, 'dy and total')
         if dtype not in (None, total.dtype):
             raise TypeError(f'dx has the type of total, {total.dtype}')
         dtype = total.dtype
-    else:
-        check_packed(total)
-        check_same_shape(dy, total.codes, 'dy and total')
-        dtype = dy.dtype if dtype is None else dtype
-    _check_types(dy.dtype, dtype)
+    _check_types(dtype, dy.dtype)
     _check_param(weight, 'weight', dy)
     rows = dy.numel() // dy.shape[-1]
     for t, name in ((mean, 'mean'), (rstd, 'rstd')):
@@ -190,24 +206,7 @@ def layer_norm_backward(
         check_same_shape(dy, grad_total, 'dy and grad_total')
         if grad_total.dtype != dtype:
             raise TypeError(f'grad_total must be {dtype}, as dx is')
-    if dy.is_cuda:
-        ext = ops._require_ext('layer_norm_backward')
-        if ext is not None:
-            packed = isinstance(total, tuple)
-            return ext.norm_backward(
-                dy.contiguous(),
-                None if packed else total.contiguous(),
-                total[0].contiguous() if packed else None,
-                total[1].contiguous() if packed else None,
-                mean.contiguous(),
-                rstd.contiguous(),
-                None if weight is None else weight.contiguous(),
-                weight is not None,
-                bias,
-                None if grad_total is None else grad_total.contiguous(),
-                dtype,
-            )
-    if not isinstance(total, torch.Tensor):
+    if packed:
         total = ref.unpack8(*total)
     dx, dw, db = ref.layer_norm_backward(
         dy, total, mean, rstd, weight, grad_total, dtype,

@@ -305,20 +305,40 @@ def test_offsets_beyond_31_bits() -> None:
 def test_refusals() -> None:
     x = rand(4, 70)
     p = ops.pack8(x)
+    with pytest.raises(TypeError):
+        ops.pack8(x.double())
+    with pytest.raises(TypeError):
+        ops.pack8(torch.zeros(4, 4, dtype=torch.int32, device='cuda'))
     with pytest.raises(ValueError):
-        ops.weight_grad8(torch.zeros(4, 5), p)
+        ops.pack8(torch.tensor(1.0, device='cuda'))
+    with pytest.raises(ValueError):
+        ops.pack8(torch.zeros(3, 0, device='cuda'))
+    with pytest.raises(TypeError):
+        ops.unpack8(p, torch.float64)
+    with pytest.raises(TypeError):
+        ops.unpack8(ops.Packed8(p.codes.int(), p.exponents))
+    for exps in (
+        p.exponents[:, :1], p.exponents[:3], p.exponents.view(2, 2, 2),
+        p.exponents.cpu(),
+    ):
+        with pytest.raises(ValueError):
+            ops.unpack8(ops.Packed8(p.codes, exps))
+        with pytest.raises(ValueError):
+            ops.weight_grad8(x, ops.Packed8(p.codes, exps))
+        with pytest.raises(ValueError):
+            ops.gelu8_backward(x, ops.Packed8(p.codes, exps))
+    with pytest.raises(ValueError):
+        ops.gelu8_forward(x, approximate='sigmoid')
+    with pytest.raises(ValueError):
+        ops.gelu8_backward(x[:, :69], p)
+    with pytest.raises(TypeError):
+        ops.gelu8_backward(x.double(), p)
     with pytest.raises(ValueError):
         ops.gelu8_backward(x.cpu(), p)
-    with pytest.raises(ValueError):
-        ops.unpack8(ops.Packed8(p.codes, p.exponents.cpu()))
-    # the extension checks for itself
-    from kfac_amd import _kfaccore as ext
-
-    with pytest.raises(RuntimeError):
-        ext.unpack8(p.codes, p.exponents[:, :1].contiguous(), F32)
-    with pytest.raises(RuntimeError):
-        ext.weight_grad8(x[:3], p.codes, p.exponents, True, F32)
-    with pytest.raises(RuntimeError):
-        ext.pack8(x.t())
-    with pytest.raises(RuntimeError):
-        ext.pack8(x.double())
+    for g in (x[:3], x.view(2, 2, 70), x.cpu()):
+        with pytest.raises(ValueError):
+            ops.weight_grad8(g, p)
+    with pytest.raises(TypeError):
+        ops.weight_grad8(x.double(), p)
+    with pytest.raises(TypeError):
+        ops.weight_grad8(x, p, dtype=torch.float64)

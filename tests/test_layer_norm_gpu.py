@@ -278,22 +278,48 @@ def test_autograd_block() -> None:
 def test_refusals() -> None:
     x, w = rand(4, 10), rand(10)
     n = ops.layer_norm_forward(x, w)
-    with pytest.raises(ValueError):
-        ops.layer_norm_forward(x, w.cpu())
-    with pytest.raises(ValueError):
-        ops.layer_norm_forward(x, residual=x.cpu())
-    with pytest.raises(ValueError):
-        ops.layer_norm_backward(x, n.total, n.mean.cpu(), n.rstd, w)
-    from kfac_amd import _kfaccore as ext
-
-    with pytest.raises(RuntimeError):
-        ext.norm_forward(x, None, w[:9], None, 1e-5, F32, False, False)
-    with pytest.raises(RuntimeError):
-        ext.norm_forward(
-            x.bfloat16(), None, None, None, 1e-5, F16, False, False,
+    for bad in (x.double(), x.int()):
+        with pytest.raises(TypeError):
+            ops.layer_norm_forward(bad)
+    for bad in (torch.tensor(1.0).cuda(), torch.zeros(3, 0).cuda()):
+        with pytest.raises(ValueError):
+            ops.layer_norm_forward(bad)
+    for bad in (w[:9], w.view(1, 10), w.cpu()):
+        with pytest.raises(ValueError):
+            ops.layer_norm_forward(x, bad)
+        with pytest.raises(ValueError):
+            ops.layer_norm_forward(x, w, bad)
+    with pytest.raises(TypeError):
+        ops.layer_norm_forward(x, w.double())
+    with pytest.raises(TypeError):
+        ops.layer_norm_forward(x, out_dtype=torch.float64)
+    with pytest.raises(TypeError):
+        ops.layer_norm_forward(x.bfloat16(), out_dtype=F16)
+    for bad in (x, x.half(), x.double()):
+        with pytest.raises(TypeError):
+            ops.layer_norm_forward(x.bfloat16(), residual=bad)
+    for bad in (x[:, :1], x.cpu()):
+        with pytest.raises(ValueError):
+            ops.layer_norm_forward(x, residual=bad)
+    args = (x, n.total, n.mean, n.rstd, w)
+    for i, bad in (
+        (0, x[:3]), (1, x[:3]), (1, x.cpu()), (2, n.mean[:3]),
+        (2, n.mean.cpu()), (3, n.rstd.view(4, 1)), (3, n.rstd.double()),
+        (4, w[:9]), (1, ops.pack8(x[:3])),
+    ):
+        with pytest.raises(ValueError):
+            ops.layer_norm_backward(*args[:i], bad, *args[i + 1:])
+    with pytest.raises(TypeError):
+        ops.layer_norm_backward(*args, dtype=BF16)
+    with pytest.raises(TypeError):
+        ops.layer_norm_backward(
+            x, ops.pack8(x), n.mean, n.rstd, dtype=torch.float64,
         )
-    with pytest.raises(RuntimeError):
-        ext.norm_backward(
-            x, x[:3].contiguous(), None, None, n.mean, n.rstd, w, True,
-            True, None, F32,
+    with pytest.raises(TypeError):
+        ops.layer_norm_backward(
+            x.half(), ops.pack8(x), n.mean, n.rstd, dtype=BF16,
         )
+    with pytest.raises(TypeError):
+        ops.layer_norm_backward(*args, grad_total=x.bfloat16())
+    with pytest.raises(ValueError):
+        ops.layer_norm_backward(*args, grad_total=x[:3])
