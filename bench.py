@@ -68,6 +68,14 @@ def parse_args() -> argparse.Namespace:
         help='LM only: precondition attention projections too (not just '
         'MLP linears) — exercises the n=3072/768 factor pipeline',
     )
+    p.add_argument(
+        '--activation-bits',
+        type=int,
+        default=None,
+        choices=[8],
+        help='LM only: keep the activations of norms, linears and GELU in 8 '
+        'bits for the backward pass',
+    )
     return p.parse_args()
 
 
@@ -109,7 +117,11 @@ def main() -> None:
         'resnet152': resnet152,
         'gptneox125m': gptneox_125m,
     }[args.model]
-    model = model_fn().to(device)
+    if args.activation_bits is not None and not is_lm:
+        raise SystemExit('--activation-bits needs --model gptneox125m')
+    model = (
+        model_fn(activation_bits=args.activation_bits) if is_lm else model_fn()
+    ).to(device)
     model.train()
     if is_lm and args.batch_size == 64:
         args.batch_size = 8  # 8 x 2048 tokens per GPU
@@ -309,6 +321,10 @@ def main() -> None:
                 'async_inverse': bool(args.async_inverse),
                 'compute_method': args.compute_method,
                 'lm_full': args.lm_full if is_lm else None,
+                'activation_bits': args.activation_bits,
+                'peak_memory_gib': (
+                    torch.cuda.max_memory_allocated() / 2**30
+                ),
                 'all_in_ms_per_step': all_in_ms_per_step,
                 'inv_phase_ms': inv_phase_ms,
                 'precond_step_ms_mean': (

@@ -223,7 +223,7 @@ class KFACBaseLayer:
             s.wait_stream(torch.cuda.current_stream(a.device))
             with torch.cuda.stream(s):
                 self.module.accumulate_a_factor(a, self._a_batch, beta, 1.0)
-            self._pending_inputs.append(a)
+            self._hold(a, s)
         else:
             self.module.accumulate_a_factor(a, self._a_batch, beta, 1.0)
         self._a_count += 1
@@ -255,10 +255,23 @@ class KFACBaseLayer:
             s.wait_stream(torch.cuda.current_stream(g.device))
             with torch.cuda.stream(s):
                 self.module.accumulate_g_factor(g, self._g_batch, beta, coeff)
-            self._pending_inputs.append(g)
+            self._hold(g, s)
         else:
             self.module.accumulate_g_factor(g, self._g_batch, beta, coeff)
         self._g_count += 1
+
+    def _hold(self, t: torch.Tensor, stream: torch.cuda.Stream) -> None:
+        """Keep ``t``'s memory until the covariance stream has read it.
+
+        The reference is dropped in clear_pending() at the step. A module
+        that keeps its input in fewer bits (``keeps_codes``) would keep the
+        whole tensor that way: its memory is given back as soon as the
+        stream is past the read.
+        """
+        if getattr(self.module.module, 'keeps_codes', False):
+            t.record_stream(stream)
+            t = t.new_empty(0)
+        self._pending_inputs.append(t)
 
     def _factor_ctx(self) -> Any:
         """Stream context for factor EMA/reduce ops.

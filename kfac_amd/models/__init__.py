@@ -3,7 +3,8 @@
 Self-contained (torchvision is not a dependency): ImageNet-style ResNets
 (resnet50/101/152 — bench.py's flagship is resnet50), CIFAR option-A
 ResNets (resnet20..1202, reference examples/vision/cifar_resnet.py), and
-a Transformer LM (examples/language).
+a Transformer LM (examples/language). LayerNorm8, Linear8 and GELU8 keep a
+transformer block's activations in 8 bits.
 """
 
 from kfac_amd.models.cifar_resnet import cifar_resnet
@@ -12,6 +13,9 @@ from kfac_amd.models.resnet import resnet101
 from kfac_amd.models.resnet import resnet152
 from kfac_amd.models.gptneox import gptneox_125m
 from kfac_amd.models.gptneox import GPTNeoXModel
+from kfac_amd.models.modules import GELU8
+from kfac_amd.models.modules import LayerNorm8
+from kfac_amd.models.modules import Linear8
 from kfac_amd.models.transformer import TransformerModel
 
 __all__ = [
@@ -22,4 +26,7 @@ __all__ = [
     'TransformerModel',
     'GPTNeoXModel',
     'gptneox_125m',
+    'LayerNorm8',
+    'Linear8',
+    'GELU8',
 ]
