@@ -172,7 +172,9 @@ class KFACEigenLayer(KFACBaseLayer):
         if self.symmetric_factors:
             da, qa = ops.eigh(a, clamp=False)
         else:
-            dac, qac = torch.linalg.eig(a)
+            # fp32 eigenvectors of a nearly symmetric factor may be off by
+            # 1e-5, as far as they differ between CPUs
+            dac, qac = torch.linalg.eig(a.to(torch.float64))
             da, qa = dac.real, qac.real
         self.qa = qa.to(self.inv_dtype)
         self.da = torch.clamp(da.to(self.inv_dtype), min=0.0)
@@ -186,7 +188,7 @@ class KFACEigenLayer(KFACBaseLayer):
         if self.symmetric_factors:
             dg, qg = ops.eigh(g, clamp=False)
         else:
-            dgc, qgc = torch.linalg.eig(g)
+            dgc, qgc = torch.linalg.eig(g.to(torch.float64))
             dg, qg = dgc.real, qgc.real
         self.qg = qg.to(self.inv_dtype)
         self.dg = torch.clamp(dg.to(self.inv_dtype), min=0.0)
