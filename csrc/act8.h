@@ -228,42 +228,76 @@ __device__ __forceinline__ void codes4(unsigned word, float s, float v[4]) {
   v[3] = code<3>(word) * s;
 }
 
+// max(|a|, |b|, |c|), NaN if one is: one instruction.
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float v;
+  asm("v_maximum3_f32 %0, |%1|, |%2|, |%3|"
+      : "=v"(v)
+      : "v"(a), "v"(b), "v"(c));
+  return v;
+}
+
 // Packs the 8 values of each lane; all lanes of a block take part. Only the
-// values from `skip` on belong to the block, up to `n` (none if n <= skip):
-// the others are not looked at, and their codes not written.
+// values from `skip` on belong to the block (0 unless PART), and none unless
+// `any`: the others are not looked at, and their codes not written. Of a row
+// that ends inside the lane's 8 the first n are written, behind them are
+// zeros.
+template <bool PART>
 __device__ __forceinline__ void pack_chunk(
     const float v[8],
+    bool any,
     int skip,
     int n,
     int8_t* codes,
     uint8_t* exponent,
     bool first) {
-  unsigned top = 0;
+  float m[8];
 #pragma unroll
-  for (int j = 0; j < kChunk; ++j) {
-    const unsigned a = __float_as_uint(v[j]) & 0x7FFFFFFF;
-    top = top > a || j < skip || j >= n ? top : a;
-  }
-  const unsigned byte = exponent_of(max_of_block(top));
+  for (int j = 0; j < kChunk; ++j) m[j] = PART && j < skip ? 0.f : v[j];
+  float top = max3_abs(m[0], m[1], m[2]);
+  top = max3_abs(top, m[3], m[4]);
+  top = max3_abs(top, m[5], m[6]);
+  top = max3_abs(top, m[7], m[7]);
+  const unsigned byte =
+      exponent_of(max_of_block(any ? __float_as_uint(top) : 0));
+  if (!any) return;
   // 2^-e; a block that holds no number gets codes of 0
   const float inv = __uint_as_float(byte == 255 ? 0u : (254 - byte) << 23);
-  unsigned c[2] = {};
+  if (byte == 248) {
+    // the one exponent that is bounded from above: 127 * 2^121
+    const float most = __uint_as_float(0x7F7E0000);
+    asm volatile("");  // a branch, not 8 operations for everyone
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) {
+      m[j] = __builtin_amdgcn_fmed3f(m[j], -most, most);
+    }
+  }
+  // The fma rounds to an integer (1.5 * 2^23 is even: ties go to even) whose
+  // low byte is the code.
+  unsigned q[8], c[2];
 #pragma unroll
   for (int j = 0; j < kChunk; ++j) {
-    // a NaN becomes -127 and is dropped below
-    const float q = fminf(fmaxf(rintf(v[j] * inv), -127.f), 127.f);
-    c[j / 4] |= ((unsigned)(int)q & 255) << j % 4 * 8;
+    q[j] = __float_as_uint(fmaf(m[j], inv, 12582912.f));
   }
-  if (byte == 255) c[0] = c[1] = 0;
-  if (skip == 0 && n >= kChunk) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const unsigned lo =
+        __builtin_amdgcn_perm(q[4 * j + 1], q[4 * j], 0x0C0C0400);
+    const unsigned hi =
+        __builtin_amdgcn_perm(q[4 * j + 3], q[4 * j + 2], 0x04000C0C);
+    c[j] = byte == 255 ? 0 : lo | hi;
+  }
+  if ((!PART || skip == 0) && n >= kChunk) {
     __builtin_memcpy(codes, c, 8);
   } else {
 #pragma unroll
     for (int j = 0; j < kChunk; ++j) {
-      if (j >= skip && j < n) codes[j] = (int8_t)(c[j / 4] >> j % 4 * 8);
+      if ((!PART || j >= skip) && j < n) {
+        codes[j] = (int8_t)(c[j / 4] >> j % 4 * 8);
+      }
     }
   }
-  if (first && n > skip) *exponent = (uint8_t)byte;
+  if (first) *exponent = (uint8_t)byte;
 }
 
 __device__ __forceinline__ void unpack8(

@@ -12,58 +12,124 @@ namespace kfac {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kRows = 2;  // that a thread takes one after the other
 
-// Rows are padded to whole blocks of lanes: unit u is chunk u % upr of row
-// u / upr, upr a multiple of 8.
-struct Unit {
-  long row;
-  int chunk;
-  int n;  // how many of the chunk's 8 values are in the row
+// A block covers 256 / L rows of L chunks, kRows times; L is a power of two,
+// so that finding a thread's place takes shifts only.
+struct Place {
+  long R;
+  int D;
+  int blocks;  // exponents a row
+  int shift;   // log2 L
 };
 
-__device__ __forceinline__ Unit unit_of(unsigned u, unsigned upr, int D) {
-  const unsigned row = u / upr;
-  const unsigned chunk = u - row * upr;
-  return {(long)row, (int)chunk, D - (int)chunk * kChunk};
+struct Chunk {
+  long row;  // the first one
+  int step;  // to the next one
+  int chunk;
+  int n;     // how many of the chunk's 8 values are in a row
+};
+
+__device__ __forceinline__ Chunk chunk_of(const Place& p) {
+  const int rows = kThreads >> p.shift;
+  const int lane = threadIdx.x & ((1 << p.shift) - 1);
+  Chunk c;
+  c.row = (long)blockIdx.y * rows * kRows + (threadIdx.x >> p.shift);
+  c.step = rows;
+  c.chunk = (blockIdx.x << p.shift) + lane;
+  c.n = p.D - c.chunk * kChunk;
+  return c;
 }
 
-template <typename T>
+// TAIL: rows may end inside a chunk.
+template <bool TAIL, typename T>
+__device__ __forceinline__ void get(const T* p, int n, float v[8]) {
+  if (TAIL) {
+    load_chunk(p, n, v);
+  } else {
+    load8(p, v);
+  }
+}
+template <bool TAIL, typename T>
+__device__ __forceinline__ void put(T* p, int n, const float v[8]) {
+  if (TAIL) {
+    store_chunk(p, n, v);
+  } else {
+    store8(p, v);
+  }
+}
+
+// All lanes of a block of 64 values call this, or none.
+template <bool TAIL>
+__device__ __forceinline__ void pack(
+    const float v[8],
+    const Place& p,
+    const Chunk& c,
+    long row,
+    int8_t* codes,
+    uint8_t* exps) {
+  const bool any = c.n > 0;
+  pack_chunk<false>(
+      v, any, 0, TAIL ? c.n : kChunk, codes + row * p.D + c.chunk * kChunk,
+      exps + row * p.blocks + c.chunk / 8, c.chunk % 8 == 0);
+}
+
+template <typename T, bool TAIL>
 __global__ __launch_bounds__(kThreads) void pack8_kernel(
     const T* __restrict__ x,
     int8_t* __restrict__ codes,
     uint8_t* __restrict__ exps,
-    unsigned units,
-    unsigned upr,
-    int D,
-    int blocks) {
-  const unsigned u = blockIdx.x * kThreads + threadIdx.x;
-  if (u >= units) return;  // whole blocks: upr is a multiple of 8
-  const Unit t = unit_of(u, upr, D);
-  const long at = t.row * D + t.chunk * kChunk;
-  float v[8];
-  load_chunk(x + at, t.n, v);
-  pack_chunk(
-      v, 0, t.n, codes + at, exps + t.row * blocks + t.chunk / 8,
-      t.chunk % 8 == 0);
+    Place p) {
+  const Chunk c = chunk_of(p);
+  float v[kRows][8] = {};
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const long row = c.row + i * c.step;
+    if (row < p.R && c.n > 0) {
+      get<TAIL>(x + row * p.D + c.chunk * kChunk, c.n, v[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const long row = c.row + i * c.step;
+    if (row < p.R) pack<TAIL>(v[i], p, c, row, codes, exps);
+  }
 }
 
-template <typename T>
+// The codes and the exponent of a chunk.
+template <bool TAIL>
+__device__ __forceinline__ void get_packed(
+    const Place& p,
+    const Chunk& c,
+    long row,
+    const int8_t* codes,
+    const uint8_t* exps,
+    float v[8]) {
+  const int8_t* at = codes + row * p.D + c.chunk * kChunk;
+  const unsigned byte = exps[row * p.blocks + c.chunk / 8];
+  if (TAIL) {
+    unpack_chunk(at, byte, c.n, v);
+  } else {
+    unpack8(at, byte, v);
+  }
+}
+
+template <typename T, bool TAIL>
 __global__ __launch_bounds__(kThreads) void unpack8_kernel(
     const int8_t* __restrict__ codes,
     const uint8_t* __restrict__ exps,
     T* __restrict__ out,
-    unsigned units,
-    unsigned upr,
-    int D,
-    int blocks) {
-  const unsigned u = blockIdx.x * kThreads + threadIdx.x;
-  if (u >= units) return;
-  const Unit t = unit_of(u, upr, D);
-  if (t.n <= 0) return;
-  const long at = t.row * D + t.chunk * kChunk;
-  float v[8];
-  unpack_chunk(codes + at, exps[t.row * blocks + t.chunk / 8], t.n, v);
-  store_chunk(out + at, t.n, v);
+    Place p) {
+  const Chunk c = chunk_of(p);
+  if (c.n <= 0) return;
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const long row = c.row + i * c.step;
+    if (row >= p.R) return;
+    float v[8];
+    get_packed<TAIL>(p, c, row, codes, exps, v);
+    put<TAIL>(out + row * p.D + c.chunk * kChunk, c.n, v);
+  }
 }
 
 // GELU: y = x * P(x) with P the normal distribution function, or its tanh
@@ -101,11 +167,10 @@ __device__ __forceinline__ float gate_of(float x) {
 
 template <bool TANH>
 __device__ __forceinline__ float gelu_of(float x) {
-  // below -100 the gate is 0: so is the result, at minus infinity too
-  if (TANH) return fmaxf(x, -100.f) * gate_of(x);
+  if (TANH) return x * gate_of(x);
   float e;
   const float q = lower_tail(x, e);
-  return fmaf(-fminf(fabsf(x), 100.f), q, fmaxf(x, 0.f));
+  return x * (x < 0.f ? q : 1.f - q);
 }
 
 template <bool TANH>
@@ -113,7 +178,7 @@ __device__ __forceinline__ float gelu_slope(float x) {
   if (TANH) {
     const float p = gate_of(x);
     // p (1 - p) is 0 beyond |x| = 30, where x^2 may overflow
-    const float c = fminf(fmaxf(x, -30.f), 30.f);
+    const float c = __builtin_amdgcn_fmed3f(x, -30.f, 30.f);
     const float slope = kGate * fmaf(3.f * kCubic * c, c, 1.f);
     return fmaf(c * p * (1.f - p), slope, p);
   }
@@ -122,7 +187,7 @@ __device__ __forceinline__ float gelu_slope(float x) {
   return fmaf(x * e, kInvSqrt2Pi, x < 0.f ? q : 1.f - q);
 }
 
-template <typename T, bool TANH>
+template <typename T, bool TANH, bool TAIL>
 __global__ __launch_bounds__(kThreads) void gelu8_fwd_kernel(
     const T* __restrict__ x,
     T* __restrict__ y,
@@ -130,68 +195,88 @@ __global__ __launch_bounds__(kThreads) void gelu8_fwd_kernel(
     uint8_t* __restrict__ in_exps,
     int8_t* __restrict__ out_codes,  // may be null
     uint8_t* __restrict__ out_exps,
-    unsigned units,
-    unsigned upr,
-    int D,
-    int blocks) {
-  const unsigned u = blockIdx.x * kThreads + threadIdx.x;
-  if (u >= units) return;
-  const Unit t = unit_of(u, upr, D);
-  const long at = t.row * D + t.chunk * kChunk;
-  const long block = t.row * blocks + t.chunk / 8;
-  const bool first = t.chunk % 8 == 0;
-  float v[8];
-  load_chunk(x + at, t.n, v);
-  if (in_codes != nullptr) {
-    pack_chunk(v, 0, t.n, in_codes + at, in_exps + block, first);
+    Place p) {
+  const Chunk c = chunk_of(p);
+  float v[kRows][8] = {};
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const long row = c.row + i * c.step;
+    if (row < p.R && c.n > 0) {
+      get<TAIL>(x + row * p.D + c.chunk * kChunk, c.n, v[i]);
+    }
   }
 #pragma unroll
-  for (int j = 0; j < kChunk; ++j) v[j] = round_to(gelu_of<TANH>(v[j]), y);
-  store_chunk(y + at, t.n, v);
-  if (out_codes != nullptr) {
-    pack_chunk(v, 0, t.n, out_codes + at, out_exps + block, first);
+  for (int i = 0; i < kRows; ++i) {
+    const long row = c.row + i * c.step;
+    if (row >= p.R) return;
+    if (in_codes != nullptr) pack<TAIL>(v[i], p, c, row, in_codes, in_exps);
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) {
+      v[i][j] = round_to(gelu_of<TANH>(v[i][j]), y);
+    }
+    if (c.n > 0) put<TAIL>(y + row * p.D + c.chunk * kChunk, c.n, v[i]);
+    if (out_codes != nullptr) {
+      pack<TAIL>(v[i], p, c, row, out_codes, out_exps);
+    }
   }
 }
 
-template <typename T, bool TANH>
+template <typename T, bool TANH, bool TAIL>
 __global__ __launch_bounds__(kThreads) void gelu8_bwd_kernel(
     const T* __restrict__ dy,
     const int8_t* __restrict__ codes,
     const uint8_t* __restrict__ exps,
     T* __restrict__ dx,
-    unsigned units,
-    unsigned upr,
-    int D,
-    int blocks) {
-  const unsigned u = blockIdx.x * kThreads + threadIdx.x;
-  if (u >= units) return;
-  const Unit t = unit_of(u, upr, D);
-  if (t.n <= 0) return;
-  const long at = t.row * D + t.chunk * kChunk;
-  float g[8], v[8];
-  load_chunk(dy + at, t.n, g);
-  unpack_chunk(codes + at, exps[t.row * blocks + t.chunk / 8], t.n, v);
+    Place p) {
+  const Chunk c = chunk_of(p);
+  if (c.n <= 0) return;
+  float g[kRows][8], v[kRows][8];
 #pragma unroll
-  for (int j = 0; j < kChunk; ++j) g[j] *= gelu_slope<TANH>(v[j]);
-  store_chunk(dx + at, t.n, g);
+  for (int i = 0; i < kRows; ++i) {
+    const long row = c.row + i * c.step;
+    if (row < p.R) {
+      get<TAIL>(dy + row * p.D + c.chunk * kChunk, c.n, g[i]);
+      get_packed<TAIL>(p, c, row, codes, exps, v[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const long row = c.row + i * c.step;
+    if (row >= p.R) return;
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) g[i][j] *= gelu_slope<TANH>(v[i][j]);
+    put<TAIL>(dx + row * p.D + c.chunk * kChunk, c.n, g[i]);
+  }
 }
 
-// Calls fn(first row, rows, units, upr) for slabs of rows whose units fit
-// 31 bits (a tensor of more than 2^34 values takes several launches).
+// Calls fn(grid, place, first row, TAIL) for slabs of rows that a grid's
+// second dimension can hold.
 template <typename Fn>
 hipError_t by_slabs(long R, int D, Fn fn) {
-  const long upr = (long)ceil_div(D, kBlock8) * 8;
-  const long most = (1L << 31) / upr - 1;
+  const int blocks = ceil_div(D, kBlock8), chunks = blocks * 8;
+  // the widest power of two that leaves no more than 1/16 of the lanes idle
+  int shift = 8;
+  while (shift > 3 &&
+         (long)(ceil_div(chunks, 1 << shift) << shift) * 15 >
+             (long)chunks * 16) {
+    --shift;
+  }
+  const int rows = (kThreads >> shift) * kRows;
+  const long most = 65535L * rows;
   for (long r = 0; r < R; r += most) {
-    const long rows = R - r < most ? R - r : most;
-    fn(r, (unsigned)(rows * upr), (unsigned)upr);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
+    const long here = R - r < most ? R - r : most;
+    const dim3 grid(
+        ceil_div(chunks, 1 << shift), (unsigned)((here + rows - 1) / rows));
+    const Place p{here, D, blocks, shift};
+    if (D % kChunk) {
+      fn(grid, p, r, std::true_type());
+    } else {
+      fn(grid, p, r, std::false_type());
+    }
+    KFAC_HIP_CHECK(hipGetLastError());
   }
   return hipSuccess;
 }
-
-unsigned grid_of(unsigned units) { return (units + kThreads - 1) / kThreads; }
 
 }  // namespace
 
@@ -203,10 +288,9 @@ hipError_t pack8_t(
     uint8_t* exps,
     long R,
     int D) {
-  const int blocks = ceil_div(D, kBlock8);
-  return by_slabs(R, D, [&](long r, unsigned units, unsigned upr) {
-    pack8_kernel<T><<<grid_of(units), kThreads, 0, s>>>(
-        x + r * D, codes + r * D, exps + r * blocks, units, upr, D, blocks);
+  return by_slabs(R, D, [&](dim3 grid, const Place& p, long r, auto tail) {
+    pack8_kernel<T, decltype(tail)::value><<<grid, kThreads, 0, s>>>(
+        x + r * D, codes + r * D, exps + r * p.blocks, p);
   });
 }
 
@@ -218,10 +302,9 @@ hipError_t unpack8_t(
     T* out,
     long R,
     int D) {
-  const int blocks = ceil_div(D, kBlock8);
-  return by_slabs(R, D, [&](long r, unsigned units, unsigned upr) {
-    unpack8_kernel<T><<<grid_of(units), kThreads, 0, s>>>(
-        codes + r * D, exps + r * blocks, out + r * D, units, upr, D, blocks);
+  return by_slabs(R, D, [&](dim3 grid, const Place& p, long r, auto tail) {
+    unpack8_kernel<T, decltype(tail)::value><<<grid, kThreads, 0, s>>>(
+        codes + r * D, exps + r * p.blocks, out + r * D, p);
   });
 }
 
@@ -237,14 +320,15 @@ hipError_t gelu8_fwd_t(
     long R,
     int D,
     bool tanh) {
-  const int blocks = ceil_div(D, kBlock8);
-  auto kernel = tanh ? gelu8_fwd_kernel<T, true> : gelu8_fwd_kernel<T, false>;
-  return by_slabs(R, D, [&](long r, unsigned units, unsigned upr) {
-    kernel<<<grid_of(units), kThreads, 0, s>>>(
+  return by_slabs(R, D, [&](dim3 grid, const Place& p, long r, auto tail) {
+    constexpr bool TAIL = decltype(tail)::value;
+    auto kernel = tanh ? gelu8_fwd_kernel<T, true, TAIL>
+                       : gelu8_fwd_kernel<T, false, TAIL>;
+    kernel<<<grid, kThreads, 0, s>>>(
         x + r * D, y + r * D, ic == nullptr ? nullptr : ic + r * D,
-        ic == nullptr ? nullptr : ie + r * blocks,
+        ic == nullptr ? nullptr : ie + r * p.blocks,
         oc == nullptr ? nullptr : oc + r * D,
-        oc == nullptr ? nullptr : oe + r * blocks, units, upr, D, blocks);
+        oc == nullptr ? nullptr : oe + r * p.blocks, p);
   });
 }
 
@@ -258,12 +342,12 @@ hipError_t gelu8_bwd_t(
     long R,
     int D,
     bool tanh) {
-  const int blocks = ceil_div(D, kBlock8);
-  auto kernel = tanh ? gelu8_bwd_kernel<T, true> : gelu8_bwd_kernel<T, false>;
-  return by_slabs(R, D, [&](long r, unsigned units, unsigned upr) {
-    kernel<<<grid_of(units), kThreads, 0, s>>>(
-        dy + r * D, codes + r * D, exps + r * blocks, dx + r * D, units, upr,
-        D, blocks);
+  return by_slabs(R, D, [&](dim3 grid, const Place& p, long r, auto tail) {
+    constexpr bool TAIL = decltype(tail)::value;
+    auto kernel = tanh ? gelu8_bwd_kernel<T, true, TAIL>
+                       : gelu8_bwd_kernel<T, false, TAIL>;
+    kernel<<<grid, kThreads, 0, s>>>(
+        dy + r * D, codes + r * D, exps + r * p.blocks, dx + r * D, p);
   });
 }
 

@@ -204,10 +204,9 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * kWave) void norm_fwd_kernel(
     for (int i = 0; i < NCH; ++i) {
       const Part p = part_of<ODD, kLanes>(lane, i, a.D);
       const long block = row * a.blocks;
-      const int n = p.any ? kChunk : 0;
       if (a.in_codes != nullptr) {
-        pack_chunk(
-            t[i], p.skip, n, lane_ptr(a.in_codes + start, p.col),
+        pack_chunk<ODD>(
+            t[i], p.any, p.skip, kChunk, lane_ptr(a.in_codes + start, p.col),
             lane_ptr(a.in_exps + block, p.chunk / 8), p.chunk % 8 == 0);
       }
 #pragma unroll
@@ -217,8 +216,8 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * kWave) void norm_fwd_kernel(
       }
       if (p.any) store8(lane_ptr(a.y + start, p.col), t[i]);
       if (a.out_codes != nullptr) {
-        pack_chunk(
-            t[i], p.skip, n, lane_ptr(a.out_codes + start, p.col),
+        pack_chunk<ODD>(
+            t[i], p.any, p.skip, kChunk, lane_ptr(a.out_codes + start, p.col),
             lane_ptr(a.out_exps + block, p.chunk / 8), p.chunk % 8 == 0);
       }
     }
@@ -508,8 +507,8 @@ __global__ __launch_bounds__(1024) void norm_fwd_long_kernel(
       float t[8];
       load_chunk(kept + start + col, n, t);
       if (a.in_codes != nullptr) {
-        pack_chunk(
-            t, 0, n, a.in_codes + start + col, a.in_exps + block,
+        pack_chunk<false>(
+            t, n > 0, 0, n, a.in_codes + start + col, a.in_exps + block,
             chunk % 8 == 0);
       }
       float w[8], b[8];
@@ -523,8 +522,8 @@ __global__ __launch_bounds__(1024) void norm_fwd_long_kernel(
       }
       store_chunk(a.y + start + col, n, t);
       if (a.out_codes != nullptr) {
-        pack_chunk(
-            t, 0, n, a.out_codes + start + col, a.out_exps + block,
+        pack_chunk<false>(
+            t, n > 0, 0, n, a.out_codes + start + col, a.out_exps + block,
             chunk % 8 == 0);
       }
     }

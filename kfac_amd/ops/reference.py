@@ -251,11 +251,9 @@ def _gelu_gate(x: torch.Tensor) -> torch.Tensor:
 def gelu(x: torch.Tensor, approximate: str) -> torch.Tensor:
     """x * P(x), P the normal distribution function or its tanh form."""
     v = x.to(torch.float32)
-    # below -100 the gate is 0: so is the result, at minus infinity too
-    low = v.clamp(min=-100)
     if approximate == 'tanh':
-        return (low * _gelu_gate(v)).to(x.dtype)
-    return (low * 0.5 * torch.erfc(-v * math.sqrt(0.5))).to(x.dtype)
+        return (v * _gelu_gate(v)).to(x.dtype)
+    return (v * 0.5 * torch.erfc(-v * math.sqrt(0.5))).to(x.dtype)
 
 
 def gelu_backward(
