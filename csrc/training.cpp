@@ -12,6 +12,8 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 
+#include <cstdlib>
+#include <cstring>
 #include <tuple>
 
 namespace {
@@ -425,6 +427,10 @@ std::tuple<Tensor, OptTensor> weight_grad8(
   const Borrowed gc = g.expect_contiguous();
   const Borrowed cc = codes.expect_contiguous(), ec = exps.expect_contiguous();
   const long M = sg.R, N = sg.D, K = sx.D;
+  // 32 of these rows are addressed with 32 bits
+  TORCH_CHECK_VALUE(
+      N < (1L << 27) && K < (1L << 27),
+      "a weight gradient takes rows of less than 2^27 values");
   OptTensor db;
   if (M == 0) {
     if (want_bias) db = zeros({N}, dtype, g);
@@ -463,9 +469,16 @@ std::tuple<Tensor, OptTensor> weight_grad8(
   return {std::move(dw), std::move(db)};
 }
 
+// KFAC_AMD_FORCE_EAGER=1, which may change while a program runs
+bool force_eager() {
+  const char* v = std::getenv("KFAC_AMD_FORCE_EAGER");
+  return v != nullptr && std::strcmp(v, "1") == 0;
+}
+
 }  // namespace
 
 void bind_training(pybind11::module& m) {
+  m.def("force_eager", &force_eager, "whether the kernels are switched off");
   m.def("pack8", &pack8, "8 bit form of a tensor's rows");
   m.def("unpack8", &unpack8, "values of an 8 bit form");
   m.def("gelu8_forward", &gelu8_forward, "GELU, input kept in 8 bits");

@@ -402,36 +402,40 @@ __global__ __launch_bounds__(256) void wgrad8_add_kernel(
   const int groups = second ? kBiasGroups : kWeightGroups;
   const int lanes = 256 / groups;
   const int group = threadIdx.x / lanes, lane = threadIdx.x % lanes;
-  const long first =
-      (long)(blockIdx.x - (second ? blocks : 0)) * sum_columns(groups);
-  const long at = first + lane * 4;
-  const int live = a.n - at < 4 ? (int)(a.n - at) : 4;
-  float s[4] = {};
-  if (live == 4) {
+  const long columns = sum_columns(groups);
+  const long step = (second ? gridDim.x - blocks : blocks) * columns;
+  for (long first = (blockIdx.x - (second ? blocks : 0)) * columns;
+       first < a.n; first += step) {
+    const long at = first + lane * 4;
+    const int live = a.n - at < 4 ? (int)(a.n - at) : 4;
+    float s[4] = {};
+    if (live == 4) {
 #pragma unroll 8
-    for (int r = group; r < a.rows; r += groups) {
-      float v[4];
-      __builtin_memcpy(v, a.parts + r * a.n + at, 16);
+      for (int r = group; r < a.rows; r += groups) {
+        float v[4];
+        __builtin_memcpy(v, a.parts + r * a.n + at, 16);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[j] += v[j];
-    }
-  } else {
+        for (int j = 0; j < 4; ++j) s[j] += v[j];
+      }
+    } else {
 #pragma unroll 4
-    for (int r = group; r < a.rows; r += groups) {
+      for (int r = group; r < a.rows; r += groups) {
 #pragma unroll
-      for (int j = 0; j < 3; ++j) {
-        if (j < live) s[j] += a.parts[r * a.n + at + j];
+        for (int j = 0; j < 3; ++j) {
+          if (j < live) s[j] += a.parts[r * a.n + at + j];
+        }
       }
     }
-  }
+    __syncthreads();  // the last round's sums have been read
 #pragma unroll
-  for (int j = 0; j < 4; ++j) lds[group * lanes * 4 + lane * 4 + j] = s[j];
-  __syncthreads();
-  for (int c = threadIdx.x; c < lanes * 4; c += 256) {
-    if (first + c >= a.n) break;
-    float sum = 0.f;
-    for (int i = 0; i < groups; ++i) sum += lds[i * lanes * 4 + c];
-    store_any(a.out, a.type, first + c, sum);
+    for (int j = 0; j < 4; ++j) lds[group * lanes * 4 + lane * 4 + j] = s[j];
+    __syncthreads();
+    for (int c = threadIdx.x; c < lanes * 4; c += 256) {
+      if (first + c >= a.n) break;
+      float sum = 0.f;
+      for (int i = 0; i < groups; ++i) sum += lds[i * lanes * 4 + c];
+      store_any(a.out, a.type, first + c, sum);
+    }
   }
 }
 
@@ -564,8 +568,8 @@ hipError_t wgrad8_add(
   const Sum bias{
       bias_sums, bias_out, bias_out == nullptr ? 0 : bias_n, bias_rows, type};
   const auto blocks_of = [](long n, int groups) {
-    const int columns = sum_columns(groups);
-    return (unsigned)((n + columns - 1) / columns);
+    const long need = (n + sum_columns(groups) - 1) / sum_columns(groups);
+    return (unsigned)(need < (1 << 20) ? need : 1 << 20);
   };
   const unsigned blocks = blocks_of(weight.n, kWeightGroups);
   const unsigned more = blocks_of(bias.n, kBiasGroups);

@@ -38,6 +38,9 @@ def _load_ext() -> Any:
     op-for-op algorithm) on the same hardware.
     """
     global _EXT, _EXT_TRIED
+    if _EXT is not None:
+        # the same variable, read in 0.1 us: os.environ takes 0.4
+        return None if _EXT.force_eager() else _EXT
     if os.environ.get('KFAC_AMD_FORCE_EAGER', '0') == '1':
         return None
     if not _EXT_TRIED:

@@ -214,7 +214,7 @@ def weight_grad8(
     input, (..., K), with as many rows. Every product is exact and sums are
     kept in float32 for each type of ``g``; the results, (N, K) and (N,),
     are rounded once to ``dtype``. Without rows they are zero. The same
-    inputs give the same bits each time.
+    inputs give the same bits each time. N and K are below 2^27.
     """
     codes, exps = packed_input
     if g.is_cuda:
