@@ -64,6 +64,15 @@ __device__ __forceinline__ float row_sum(float v, float* lds, int& at) {
   return s;
 }
 
+// 1 / sqrt(v), a Newton step behind the instruction's 1 ulp: a row's values
+// share this error, and where they round to 16 bits it decides for all.
+__device__ __forceinline__ float reciprocal_root(float v) {
+  const float r = rsqrtf(v);
+  const float left = fmaf(-v * r, r, 1.f);
+  // no step from or to 0 and infinity
+  return fabsf(left) < 1.f ? fmaf(0.5f * r, left, r) : r;
+}
+
 struct Param {
   const void* p;  // may be null
   int type;
@@ -147,7 +156,6 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * kWave) void norm_fwd_kernel(
   int at = 0;
   const int lane0 = threadIdx.x % kLanes;
   const int group = group_of(kLanes);
-  const float mean_of = 1.f / a.D;
   float w[NCH][8], b[NCH][8];
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
@@ -194,8 +202,8 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * kWave) void norm_fwd_kernel(
         square += c * c;
       }
     }
-    const float var = row_sum<W>(square, lds, at) * mean_of;
-    const float rstd = rsqrtf(var + a.eps);
+    const float var = row_sum<W>(square, lds, at) / a.D;
+    const float rstd = reciprocal_root(var + a.eps);
     if (lane == 0) {
       a.mean[row] = mean;
       a.rstd[row] = rstd;
@@ -554,7 +562,7 @@ __global__ __launch_bounds__(1024) void norm_fwd_long_kernel(
       square += part;
     }
     const float var = row_sum<16>(square, lds, at) / a.D;
-    const float rstd = rsqrtf(var + a.eps);
+    const float rstd = reciprocal_root(var + a.eps);
     if (threadIdx.x == 0) {
       a.mean[row] = mean;
       a.rstd[row] = rstd;
