@@ -389,46 +389,39 @@ __global__ __launch_bounds__(WN * WK * kWave) void wgrad8_kernel(WGrad a) {
   }
 }
 
-// One sum over rows: out[i] = sum over r < rows of parts[r][i], i < n.
+// One sum over rows: out[i] = sum over r < rows of parts[r][i], i < n. A
+// block's 256 threads take 4 columns each, in `groups` that each take every
+// groups-th row: a thread waits for each few rows that it reads, and there
+// are up to some 30 of the weight's sum, a few hundred of the bias's.
 struct Sum {
   const float* parts;
   void* out;
   long n;
   int rows;
   int type;
+  int groups;
+  unsigned blocks;
 };
 
-// Columns of a block: 4 a thread, with its 256 threads in `groups` that each
-// take every groups-th row.
-__host__ __device__ constexpr int sum_columns(int groups) {
-  return 1024 / groups;
-}
-constexpr int kWeightGroups = 4, kBiasGroups = 32;
-
-// Two sums in a launch, the weight's in the first `blocks` blocks, the
-// bias's behind them. The rows of a column are shared by 4 and by 32
-// threads: there are up to some 30 rows of the weight's sum, a few hundred
-// of the bias's, and a thread waits for each few that it reads.
+// Two sums in a launch, the weight's in the first blocks, the bias's behind
+// them.
 __global__ __launch_bounds__(256) void wgrad8_add_kernel(
     Sum weight,
-    unsigned blocks,
     Sum bias) {
   __shared__ float lds[1024];
-  const bool second = blockIdx.x >= blocks;
+  const bool second = blockIdx.x >= weight.blocks;
   const Sum a = second ? bias : weight;
-  const int groups = second ? kBiasGroups : kWeightGroups;
-  const int lanes = 256 / groups;
+  const unsigned block = blockIdx.x - (second ? weight.blocks : 0);
+  const int lanes = 256 / a.groups, columns = lanes * 4;
   const int group = threadIdx.x / lanes, lane = threadIdx.x % lanes;
-  const long columns = sum_columns(groups);
-  const long step = (second ? gridDim.x - blocks : blocks) * columns;
-  for (long first = (blockIdx.x - (second ? blocks : 0)) * columns;
-       first < a.n; first += step) {
+  for (long first = (long)block * columns; first < a.n;
+       first += (long)a.blocks * columns) {
     const long at = first + lane * 4;
     const int live = a.n - at < 4 ? (int)(a.n - at) : 4;
     float s[4] = {};
     if (live == 4) {
 #pragma unroll 8
-      for (int r = group; r < a.rows; r += groups) {
+      for (int r = group; r < a.rows; r += a.groups) {
         float v[4];
         __builtin_memcpy(v, a.parts + r * a.n + at, 16);
 #pragma unroll
@@ -436,21 +429,28 @@ __global__ __launch_bounds__(256) void wgrad8_add_kernel(
       }
     } else {
 #pragma unroll 4
-      for (int r = group; r < a.rows; r += groups) {
+      for (int r = group; r < a.rows; r += a.groups) {
 #pragma unroll
         for (int j = 0; j < 3; ++j) {
           if (j < live) s[j] += a.parts[r * a.n + at + j];
         }
       }
     }
+    if (a.groups == 1) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (j < live) store_any(a.out, a.type, at + j, s[j]);
+      }
+      continue;
+    }
     __syncthreads();  // the last round's sums have been read
 #pragma unroll
-    for (int j = 0; j < 4; ++j) lds[group * lanes * 4 + lane * 4 + j] = s[j];
+    for (int j = 0; j < 4; ++j) lds[group * columns + lane * 4 + j] = s[j];
     __syncthreads();
-    for (int c = threadIdx.x; c < lanes * 4; c += 256) {
+    for (int c = threadIdx.x; c < columns; c += 256) {
       if (first + c >= a.n) break;
       float sum = 0.f;
-      for (int i = 0; i < groups; ++i) sum += lds[i * lanes * 4 + c];
+      for (int i = 0; i < a.groups; ++i) sum += lds[i * columns + c];
       store_any(a.out, a.type, first + c, sum);
     }
   }
@@ -581,17 +581,24 @@ hipError_t wgrad8_add(
     long bias_n,
     void* bias_out,
     int type) {
-  const Sum weight{sums, out, out == nullptr ? 0 : n, splits, type};
-  const Sum bias{
-      bias_sums, bias_out, bias_out == nullptr ? 0 : bias_n, bias_rows, type};
-  const auto blocks_of = [](long n, int groups) {
-    const long need = (n + sum_columns(groups) - 1) / sum_columns(groups);
-    return (unsigned)(need < (1 << 20) ? need : 1 << 20);
+  const auto sum_of = [&](const float* parts, void* o, long n, int rows) {
+    Sum a{parts, o, o == nullptr ? 0 : n, rows, type, 1, 0};
+    // 12 rows a thread at most, and two blocks for each compute unit as long
+    // as a thread has 2 rows or more
+    while (a.groups < 32 &&
+           (a.groups * 12 < rows ||
+            (a.n * a.groups < 512L * 1024 && a.groups * 4 <= rows))) {
+      a.groups *= 2;
+    }
+    const long columns = 1024 / a.groups;
+    const long need = (a.n + columns - 1) / columns;
+    a.blocks = (unsigned)(need < (1 << 20) ? need : 1 << 20);
+    return a;
   };
-  const unsigned blocks = blocks_of(weight.n, kWeightGroups);
-  const unsigned more = blocks_of(bias.n, kBiasGroups);
-  if (blocks + more == 0) return hipSuccess;
-  wgrad8_add_kernel<<<blocks + more, 256, 0, s>>>(weight, blocks, bias);
+  const Sum weight = sum_of(sums, out, n, splits);
+  const Sum bias = sum_of(bias_sums, bias_out, bias_n, bias_rows);
+  if (weight.blocks + bias.blocks == 0) return hipSuccess;
+  wgrad8_add_kernel<<<weight.blocks + bias.blocks, 256, 0, s>>>(weight, bias);
   return hipGetLastError();
 }
 
