@@ -222,6 +222,52 @@ def test_linear8_training_step() -> None:
     plain.assert_within(db, *exact['db'])
 
 
+def test_expanded_gradient() -> None:
+    x = rand(30, 100).requires_grad_()
+    w, b = rand(70, 100).requires_grad_(), rand(70).requires_grad_()
+    y, packed = ops.gelu8(x, packed_output=True)
+    ops.linear8(y, w, b, packed=packed).sum().backward()
+    g = torch.ones(30, 70, device='cuda')
+    want = plain.weight_grads(g, plain.values8(y.detach()))
+    plain.assert_within(w.grad, *want['dw'])
+    plain.assert_within(b.grad, *want['db'])
+    dy = (g.double() @ w.detach().double()).float()
+    x8 = plain.values8(x.detach())
+    slope = plain.gelu_slope(x8, 'none')
+    # 70 additions in dy, 16 roundings in the slope
+    off = plain.UNIT * (
+        (70 + 4) * (g.double() @ w.detach().double().abs()) * slope.abs()
+        + 16 * dy.double().abs() * (1 + x8.abs())
+    )
+    plain.assert_within(x.grad, dy.double() * slope, off)
+
+
+def test_two_threads_and_streams() -> None:
+    import threading
+
+    x, g = rand(2000, 512), rand(2000, 300)
+    want = ops.weight_grad8(g, ops.pack8(x))
+    torch.cuda.synchronize()
+    results: dict[int, list] = {}
+
+    def work(i: int) -> None:
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            got = [ops.weight_grad8(g, ops.pack8(x)) for _ in range(20)]
+            stream.synchronize()
+        results[i] = got
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(results) == 4
+    for got in results.values():
+        for dw, db in got:
+            assert torch.equal(dw, want[0]) and torch.equal(db, want[1])
+
+
 def test_another_stream() -> None:
     x, g = rand(500, 256), rand(500, 300)
     p = ops.pack8(x)

@@ -19,7 +19,7 @@ PAIRS = [
 ]
 # around the widths where a row takes more lanes, and beyond registers
 WIDTHS = [
-    1, 2, 7, 8, 63, 65, 256, 511, 512, 513, 768, 1001, 1024, 1025, 2047,
+    1, 2, 7, 8, 9, 15, 63, 65, 71, 129, 256, 511, 512, 513, 768, 1001, 1024, 1025, 2047,
     2048, 2049, 4096, 4097, 8192, 8193, 16384, 16385, 20001, 33000,
 ]
 
@@ -273,6 +273,21 @@ def test_autograd_block() -> None:
     assert torch.equal(dr, dx.bfloat16())
     plain.assert_within(dw, *want['dw'])
     plain.assert_within(db, *want['db'])
+
+
+def test_expanded_gradient() -> None:
+    # what the backward pass of a sum hands over: strides of 0
+    x = rand(30, 100).requires_grad_()
+    w, b = rand(100).requires_grad_(), rand(100).requires_grad_()
+    ops.layer_norm(x, w, b).y.sum().backward()
+    n = ops.layer_norm_forward(x.detach(), w.detach(), b.detach())
+    want = plain.norm_grads(
+        torch.ones(30, 100, device='cuda'), n.total, n.mean, n.rstd,
+        w.detach(), None,
+    )
+    plain.assert_within(x.grad, *want['dx'])
+    plain.assert_within(w.grad, *want['dw'])
+    plain.assert_within(b.grad, *want['db'])
 
 
 def test_refusals() -> None:
