@@ -98,6 +98,26 @@ struct Raw {
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = load16(p + i * 4);
   }
+  // The same where only the first `left` may be there; v is clear.
+  __device__ __forceinline__ void load(const T* p, long left) {
+    if (left >= kChunk) {
+      load(p);
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < kChunk - 1; ++j) {
+      if (j >= left) continue;
+      if (sizeof(T) == 4) {
+        unsigned w;
+        __builtin_memcpy(&w, p + j, 4);
+        v[j * sizeof(T) / 16][j % 4] = w;
+      } else {
+        unsigned short h;
+        __builtin_memcpy(&h, p + j, 2);
+        v[0][j / 2] |= (unsigned)h << j % 2 * 16;
+      }
+    }
+  }
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = (u32x4)(0u);

@@ -442,7 +442,7 @@ std::tuple<Tensor, OptTensor> weight_grad8(
   by_type(g.scalar_type(), [&](auto t) {
     using T = decltype(t);
     const auto plan = kfac::wgrad8_plan<T>(M, sg.D, sx.D);
-    const long rows = (long)plan.splits * plan.tiles_k;
+    const long rows = (long)plan.splits * plan.bias_tiles;
     // a single fp32 sum is the result itself; the others share a workspace
     const bool direct = plan.splits == 1 && dtype == torch::kFloat32;
     const bool bias_direct = rows == 1 && dtype == torch::kFloat32;

@@ -58,11 +58,12 @@ struct WGradPlan {
   bool large;            // tiles
   int splits;            // of the tokens
   int tiles_n, tiles_k;  // of the output
+  int bias_tiles;        // of a row, which share the bias's sum
   long rows;             // tokens of a split
 };
 template <typename TG>
 WGradPlan wgrad8_plan(long M, int N, int K);
-// sums: [splits][N][K]; bias: [splits * tiles_k][N], may be null
+// sums: [splits][N][K]; bias: [splits * bias_tiles][N], may be null
 template <typename TG>
 hipError_t wgrad8_t(
     hipStream_t, const TG* g, const int8_t* codes, const uint8_t* exps,

@@ -39,10 +39,11 @@ struct WGrad {
   const int8_t* codes;   // [M][K]
   const uint8_t* exps;   // [M][blocks]
   float* out;            // [S][N][K]
-  float* bias;           // [S * tiles_k][N], may be null
+  float* bias;           // [S * bias_tiles][N], may be null
   long M;
   int N, K, blocks;
   int tiles_n, tiles_k;
+  int bias_tiles;  // tiles of a row that share the bias's sum
   long rows;  // tokens of a split, a multiple of the stage
 };
 
@@ -138,7 +139,7 @@ __global__ __launch_bounds__(WN * WK * kWave) void wgrad8_kernel(WGrad a) {
   // its row's end are values of the next rows, for columns that nothing is
   // stored of, so these have to be there: 7 and 15 values of them.
   int fast = (int)((m1 - m0) / BM);
-  while (fast > 0) {
+  while (fast > 0 && (a.N % 8 != 0 || a.K % 16 != 0)) {
     const long rest = a.M - m0 - (long)fast * BM;
     if (rest * a.N >= 7 && rest * a.K >= 15) break;
     --fast;
@@ -251,9 +252,10 @@ __global__ __launch_bounds__(WN * WK * kWave) void wgrad8_kernel(WGrad a) {
       __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);  // load
     }
   };
-  // the tiles of a row share the work of the bias's sum
+  // the first tiles of a row share the work of the bias's sum
+  const bool sums_bias = a.bias != nullptr && tile.k < a.bias_tiles;
   const auto add_bias = [&](const short* gl, int stage) {
-    if (a.bias == nullptr || stage % a.tiles_k != tile.k) return;
+    if (!sums_bias || stage % a.bias_tiles != tile.k) return;
 #pragma unroll
     for (int i = 0; i < GC * NP; ++i) {
       const int row = g_row + i % GC * kGDown;
@@ -286,10 +288,10 @@ __global__ __launch_bounds__(WN * WK * kWave) void wgrad8_kernel(WGrad a) {
     __syncthreads();
     read(lds, 0);
   }
-  for (int stage = 0; stage < fast; ++stage) {
+  for (int stage = 0; stage < fast - 1; ++stage) {
     const short* image = lds + (stage & 1) * kImage;
     short* next = lds + ((stage + 1) & 1) * kImage;
-    // past the end the last stage is loaded again, and not used
+    // in the last round the last stage is loaded again, and not used
     const int then = stage + 2 < fast ? stage + 2 : fast - 1;
     add_bias(image, stage);
 #pragma unroll
@@ -319,47 +321,58 @@ __global__ __launch_bounds__(WN * WK * kWave) void wgrad8_kernel(WGrad a) {
     multiply(kQ - 1);
     interleave();
   }
-  for (int stage = fast; stage < stages; ++stage) {
-    // the end of the tokens: every value is checked
+  const auto load_end = [&](int stage) {
     const long m = m0 + (long)stage * BM;
-    __syncthreads();
-#pragma unroll 1
-    for (int c = tid; c < BM * BN / 8; c += kT) {
-      const int row = c / (BN / 8), col = c % (BN / 8) * 8;
-      float v[8];
-      load_chunk(
-          (const TG*)a.g + (m + row) * a.N + n0 + col,
-          m + row < m1 ? a.N - n0 - col : 0, v);
 #pragma unroll
-      for (int p = 0; p < NP; ++p) {
-        unsigned part[4];
-        take_part(v, part);
-        __builtin_memcpy(
-            lds + p * BM * BN + slot<BN>(row, col / 8) * 8, part, 16);
+    for (int i = 0; i < GC; ++i) {
+      const long row = m + g_row + i * kGDown;
+      const long left = (a.M - row) * a.N - (n0 + gc);
+      gv[i].clear();
+      if (row < m1) {
+        gv[i].load((const TG*)a.g + row * a.N + n0 + gc, left);
       }
     }
-#pragma unroll 1
-    for (int c = tid; c < BM * BK / 8; c += kT) {
-      const int row = c / (BK / 8), col = c % (BK / 8) * 8;
-      const int n = m + row < m1 ? a.K - k0 - col : 0;
-      float v[8] = {};
-      if (n > 0) {
-        const long at = (m + row) * a.K + k0 + col;
-        unpack_chunk(
-            a.codes + at,
-            a.exps[(m + row) * a.blocks + (k0 + col) / kBlock8], n, v);
-      }
-      unsigned h[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) h[j] = high_halves(v[2 * j], v[2 * j + 1]);
-      __builtin_memcpy(
-          lds + NP * BM * BN + slot<BK>(row, col / 8) * 8, h, 16);
+    for (int i = 0; i < XC; ++i) {
+      const long row = m + x_row + i * kXDown;
+      const long left = (a.M - row) * a.K - (k0 + xc);
+      const int8_t* p = a.codes + row * a.K + k0 + xc;
+      xv[i] = (u32x4)(0u);
+      xe[i] = 1;
+      if (row < m1) {
+        xe[i] = a.exps[row * a.blocks + (k0 + xc) / kBlock8];
+        if (left >= 16) {
+          xv[i] = load16(p);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 15; ++j) {
+            if (j < left) xv[i][j / 4] |= (unsigned)(uint8_t)p[j] << j % 4 * 8;
+          }
+        }
+      }
     }
-    __syncthreads();
-    add_bias(lds, stage);
+  };
+  // The last whole stage, whose image is there, and the end of the tokens:
+  // rows behind it are zero, and what a chunk reads behind its row's end may
+  // be missing.
+  for (int stage = fast > 0 ? fast - 1 : 0; stage < stages; ++stage) {
+    const short* image = lds;
+    if (stage < fast) {
+      image += (stage & 1) * kImage;
+    } else {
+      load_end(stage);
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < GC; ++i) put_g(i, lds);
+#pragma unroll
+      for (int i = 0; i < XC; ++i) put_x(i, lds + NP * BM * BN);
+      __syncthreads();
+      read(lds, 0);
+    }
+    add_bias(image, stage);
 #pragma unroll
     for (int q = 0; q < kQ; ++q) {
-      read(lds, q);
+      if (q + 1 < kQ) read(image, q + 1);
       multiply(q);
     }
   }
@@ -378,7 +391,7 @@ __global__ __launch_bounds__(WN * WK * kWave) void wgrad8_kernel(WGrad a) {
       }
     }
   }
-  if (a.bias != nullptr) {
+  if (sums_bias) {
     // the threads that share columns, added in their order
     float* part = (float*)lds;
     __syncthreads();
@@ -389,7 +402,7 @@ __global__ __launch_bounds__(WN * WK * kWave) void wgrad8_kernel(WGrad a) {
       float s = 0.f;
       for (int i = 0; i < kGDown; ++i) s += part[i * BN + c];
       if (n0 + c < a.N) {
-        a.bias[((long)tile.split * a.tiles_k + tile.k) * a.N + n0 + c] = s;
+        a.bias[((long)tile.split * a.bias_tiles + tile.k) * a.N + n0 + c] = s;
       }
     }
   }
@@ -538,7 +551,12 @@ void consider(long M, int N, int K, WGradPlan& best, float& best_time) {
     }
     if (time < best_time) {
       best_time = time;
-      best = {LARGE, (int)s, (int)tiles_n, (int)tiles_k, per * C::BM};
+      // One tile does the bias's sum alone where that saves the second
+      // launch: some 10 % of its stages against 2.5 us.
+      const bool alone = s == 1 && per <= 16;
+      const long share = alone ? 1 : per < tiles_k ? per : tiles_k;
+      best = {LARGE, (int)s, (int)tiles_n, (int)tiles_k, (int)share,
+              per * C::BM};
     }
   }
 }
@@ -565,7 +583,7 @@ hipError_t wgrad8_t(
     float* sums,
     float* bias) {
   WGrad a{g,    codes, exps, sums, bias, M, N, K, ceil_div(K, kBlock8),
-          plan.tiles_n, plan.tiles_k, plan.rows};
+          plan.tiles_n, plan.tiles_k, plan.bias_tiles, plan.rows};
   const unsigned grid = (unsigned)plan.splits * plan.tiles_n * plan.tiles_k;
   const auto go = [&](auto large) {
     using C = Cut<TG, decltype(large)::value>;
