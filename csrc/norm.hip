@@ -145,7 +145,7 @@ __device__ __forceinline__ Part part_of(int lane, int i, int D) {
   return p;
 }
 
-// The lane's number, new to the compiler in each round of a loop: it would
+// The lane's number, new to the compiler in each turn of a loop: it would
 // keep a 64 bit address a lane for each tensor otherwise, and spill.
 __device__ __forceinline__ int fresh(int lane) {
   asm volatile("" : "+v"(lane));
@@ -713,15 +713,15 @@ hipError_t by_width(int D, Fn fn) {
 
 }  // namespace
 
-// Blocks of the backward pass. A few rounds are left to a single block, which
-// then writes the gradients itself: a second launch takes 2 to 3 us, a round 1
+// Blocks of the backward pass. A few turns are left to a single block, which
+// then writes the gradients itself: a second launch takes 2 to 3 us, a turn 1
 // us of up to 512 values, 1.7 of 1024 and 3.5 of 8192.
 static int norm_bwd_blocks(long R, int D) {
   if (is_long(D)) return (int)(R < kLongSplit ? R : kLongSplit);
   const long need = (R + rows_of_block(D) - 1) / rows_of_block(D);
   if (need <= (D <= 512 ? 4 : D <= 4096 ? 2 : 1)) return 1;
-  const long rounds = (need + 255) / 256;  // the same for each block
-  return (int)((need + rounds - 1) / rounds);
+  const long turns = (need + 255) / 256;  // the same for each block
+  return (int)((need + turns - 1) / turns);
 }
 
 int norm_bwd_partials(long R, int D) {
