@@ -10,7 +10,8 @@
 //
 // Both passes are bound by memory, so a row is read once: it stays in
 // registers between its sums and its outputs, 8 values a lane and chunk,
-// one wave a row up to 1024 values, 4, 8 or 16 up to 2048, 4096 or 16384. The
+// one wave a row up to 1024 values, 4, 8 or 16 up to 2048, 4096 or 16384 (the
+// forward pass by half for lengths that are no multiple of 8). The
 // variance is the mean of the centred squares of those registers, never a
 // difference of two large sums. The backward pass keeps dw and db of its
 // rows in registers too and writes one partial row a block; a second kernel
@@ -18,7 +19,7 @@
 // to run. Rows longer than 16384 (or shorter than 8) take the kernels at the
 // end of the file, which read a row once for each of its sums.
 //
-// Measured: forward 16384 x 8192 bf16 101 us (5.3 TB/s), 16384 x 768 fp32 and
+// Measured: forward 16384 x 8192 bf16 99 us (5.4 TB/s), 16384 x 768 fp32 and
 // a bf16 residual to bf16 and two 8 bit forms 35 us (5.0 TB/s); backward 146
 // to 159 us (5.1 to 5.5 TB/s) and, from 8 bits, 28 us (4.9 TB/s), with 5 us
 // for the parameters' sums. A copy of 1 GiB reaches 5.2 TB/s.
@@ -134,15 +135,28 @@ struct Part {
   bool any;
 };
 
-template <bool ODD, int LANES>
+template <bool ODD, int LANES, int NCH>
 __device__ __forceinline__ Part part_of(int lane, int i, int D) {
   Part p;
   p.chunk = lane + i * LANES;
   const int col = p.chunk * kChunk;
-  p.any = col < D;
-  p.skip = ODD && p.any && col > D - kChunk ? col - (D - kChunk) : 0;
+  // rows reach into the last of a lane's chunks, see by_width
+  const bool whole = i + 1 < NCH;
+  p.any = whole || col < D;
+  p.skip = ODD && !whole && p.any && col > D - kChunk ? col - (D - kChunk) : 0;
   p.col = p.any ? col - p.skip : 0;
   return p;
+}
+
+// How many of the kSpan columns that a wave's last chunks cover are in the
+// row: kSpan or more if all are, 0 or less if the wave is right of its end.
+constexpr int kSpan = kWave * kChunk;
+
+template <int W, int NCH>
+__device__ __forceinline__ int columns_of(int D) {
+  const int wave =
+      W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  return D - ((NCH - 1) * W + wave) * kSpan;
 }
 
 // The lane's number, new to the compiler in each turn of a loop: it would
@@ -164,23 +178,30 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * kWave) void norm_fwd_kernel(
   float w[NCH][8], b[NCH][8];
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
-    const Part p = part_of<ODD, kLanes>(lane0, i, a.D);
+    const Part p = part_of<ODD, kLanes, NCH>(lane0, i, a.D);
 #pragma unroll
     for (int j = 0; j < kChunk; ++j) w[i][j] = 1.f, b[i][j] = 0.f;
     if (a.w.p != nullptr) load_any(a.w, 0, p.col, w[i]);
     if (a.b.p != nullptr) load_any(a.b, 0, p.col, b[i]);
   }
+  const int columns = columns_of<W, NCH>(a.D);
   for (long base = (long)blockIdx.x * G; base < a.R;
        base += (long)gridDim.x * G) {
     const long row = base + group;
     if (W == 1 && row >= a.R) return;
+    if (NCH == 1 && W > 1 && columns <= 0) {
+      // right of the row's end: only keeps the others company
+      row_sum<W>(0.f, lds, at);
+      row_sum<W>(0.f, lds, at);
+      continue;
+    }
     const long start = row * a.D;
     const int lane = fresh(lane0);
     float t[NCH][8];
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const Part p = part_of<ODD, kLanes>(lane, i, a.D);
+      const Part p = part_of<ODD, kLanes, NCH>(lane, i, a.D);
       load8(lane_ptr(a.x + start, p.col), t[i]);
       if (a.r.p != nullptr) {
         float r[8];
@@ -191,20 +212,33 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * kWave) void norm_fwd_kernel(
         }
         if (p.any) store8(lane_ptr(a.total + start, p.col), t[i]);
       }
+      if (i + 1 < NCH || columns >= kSpan) {
 #pragma unroll
-      for (int j = 0; j < kChunk; ++j) {
-        sum += p.any && j >= p.skip ? t[i][j] : 0.f;
+        for (int j = 0; j < kChunk; ++j) sum += t[i][j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) {
+          sum += p.any && j >= p.skip ? t[i][j] : 0.f;
+        }
       }
     }
     const float mean = row_sum<W>(sum, lds, at) / a.D;
     float square = 0.f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const Part p = part_of<ODD, kLanes>(lane, i, a.D);
+      const Part p = part_of<ODD, kLanes, NCH>(lane, i, a.D);
+      if (i + 1 < NCH || columns >= kSpan) {
 #pragma unroll
-      for (int j = 0; j < kChunk; ++j) {
-        const float c = p.any && j >= p.skip ? t[i][j] - mean : 0.f;
-        square += c * c;
+        for (int j = 0; j < kChunk; ++j) {
+          const float c = t[i][j] - mean;
+          square += c * c;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) {
+          const float c = p.any && j >= p.skip ? t[i][j] - mean : 0.f;
+          square += c * c;
+        }
       }
     }
     const float var = row_sum<W>(square, lds, at) / a.D;
@@ -215,7 +249,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * kWave) void norm_fwd_kernel(
     }
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const Part p = part_of<ODD, kLanes>(lane, i, a.D);
+      const Part p = part_of<ODD, kLanes, NCH>(lane, i, a.D);
       const long block = row * a.blocks;
       if (a.in_codes != nullptr) {
         pack_chunk<ODD>(
@@ -295,7 +329,7 @@ struct KeptRow {
     rstd = a.rstd[row];
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const Part p = part_of<ODD, LANES>(lane, i, a.D);
+      const Part p = part_of<ODD, LANES, NCH>(lane, i, a.D);
       dy[i].load(lane_ptr(a.dy + start, p.col));
       if (KEPT8) {
         const uint8_t* e = a.exps + row * a.blocks;
@@ -336,10 +370,10 @@ template <typename TX, typename TY, int NCH, int W, bool ODD, bool KEPT8>
 __global__ __launch_bounds__(1024) void norm_bwd_kernel(Backward<TX, TY> a) {
   constexpr int kLanes = W * kWave;
   constexpr int G = 16 / W;                     // rows of a block
-  constexpr int kSpan = kLanes * kChunk * NCH;  // columns of a group
+  constexpr int kAll = kLanes * kChunk * NCH;   // columns of a group
   __shared__ float lds[32];
   __shared__ __attribute__((aligned(16))) float
-      parts[G > 1 ? 2 * G * kSpan : 4];
+      parts[G > 1 ? 2 * G * kAll : 4];
   int at = 0;
   const int lane0 = threadIdx.x % kLanes;
   const int group = group_of(kLanes);
@@ -347,7 +381,7 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(Backward<TX, TY> a) {
   float w[NCH][8], dw[NCH][8], db[NCH][8];
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
-    const Part p = part_of<ODD, kLanes>(lane0, i, a.D);
+    const Part p = part_of<ODD, kLanes, NCH>(lane0, i, a.D);
 #pragma unroll
     for (int j = 0; j < kChunk; ++j) {
       w[i][j] = 1.f;
@@ -381,14 +415,14 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(Backward<TX, TY> a) {
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const Part p = part_of<ODD, kLanes>(lane, i, a.D);
+      const Part p = part_of<ODD, kLanes, NCH>(lane, i, a.D);
       dy[i] = next.dy[i];
       next.template values<ODD, KEPT8>(i, p, h[i]);
     }
     if (a.dt != nullptr) {
 #pragma unroll
       for (int i = 0; i < NCH; ++i) {
-        const Part p = part_of<ODD, kLanes>(lane, i, a.D);
+        const Part p = part_of<ODD, kLanes, NCH>(lane, i, a.D);
         dt[i].load(lane_ptr(a.dt + start, p.col));
       }
     } else {
@@ -402,7 +436,7 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(Backward<TX, TY> a) {
     }
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const Part p = part_of<ODD, kLanes>(lane, i, a.D);
+      const Part p = part_of<ODD, kLanes, NCH>(lane, i, a.D);
       float g[8];
       dy[i].values(g);
 #pragma unroll
@@ -422,7 +456,7 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(Backward<TX, TY> a) {
     s2 = row_sum<W>(s2, lds, at) * mean_of;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const Part p = part_of<ODD, kLanes>(lane, i, a.D);
+      const Part p = part_of<ODD, kLanes, NCH>(lane, i, a.D);
       float g[8], d[8];
       dy[i].values(g);
       dt[i].values(d);
@@ -449,7 +483,7 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(Backward<TX, TY> a) {
     float* mine = a.partial + (long)blockIdx.x * 2 * a.D;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const Part p = part_of<ODD, kLanes>(lane0, i, a.D);
+      const Part p = part_of<ODD, kLanes, NCH>(lane0, i, a.D);
       if (!p.any) continue;
       if (!single && p.skip == 0) {
         store8(mine + p.col, dw[i]);
@@ -471,9 +505,9 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(Backward<TX, TY> a) {
   const int last = ODD ? a.D / kChunk * kChunk : a.D;
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
-    float* mine = parts + group * kSpan + (lane0 + i * kLanes) * kChunk;
+    float* mine = parts + group * kAll + (lane0 + i * kLanes) * kChunk;
     store8(mine, dw[i]);
-    store8(mine + G * kSpan, db[i]);
+    store8(mine + G * kAll, db[i]);
   }
   __syncthreads();
   for (int c = threadIdx.x; c < 2 * a.D; c += 1024) {
@@ -481,7 +515,7 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(Backward<TX, TY> a) {
     const int at = col < last ? col : col + last - (a.D - kChunk);
     float s = 0.f;
 #pragma unroll
-    for (int g = 0; g < G; ++g) s += parts[(which * G + g) * kSpan + at];
+    for (int g = 0; g < G; ++g) s += parts[(which * G + g) * kAll + at];
     put(which, col, s);
   }
 }
@@ -692,20 +726,28 @@ int rows_of_block(int D) {
 }
 
 // Calls fn with the kernel's template parameters (chunks of a lane, waves of
-// a row, odd length) as types.
-template <typename Fn>
+// a row, odd length) as types. Rows reach into the last chunk: part_of counts
+// on that. With HALVED the rows of odd lengths take half the waves and two
+// chunks a lane where they would take 4 to 16 waves: they start at any
+// alignment, such loads take longer, and more of these rows are under way at
+// a time (forward, 6898 x 6697 bf16: 51 us, 72 with 16 waves; 6696: 42 us and
+// 41, and 57 to 60 with an 8 bit form, so that other rows keep one chunk).
+template <bool HALVED, typename Fn>
 hipError_t by_width(int D, Fn fn) {
   const auto go = [&](auto odd) {
+    constexpr int kHalf = HALVED && decltype(odd)::value ? 2 : 1;
     using I1 = std::integral_constant<int, 1>;
     using I2 = std::integral_constant<int, 2>;
-    using I4 = std::integral_constant<int, 4>;
-    using I8 = std::integral_constant<int, 8>;
     using I16 = std::integral_constant<int, 16>;
+    using Chunks = std::integral_constant<int, kHalf>;
+    using W4 = std::integral_constant<int, 4 / kHalf>;
+    using W8 = std::integral_constant<int, 8 / kHalf>;
+    using W16 = std::integral_constant<int, 16 / kHalf>;
     return D <= 512 ? fn(I1(), I1(), odd)
         : D <= 1024 ? fn(I2(), I1(), odd)
-        : D <= 2048 ? fn(I1(), I4(), odd)
-        : D <= 4096 ? fn(I1(), I8(), odd)
-        : D <= 8192 ? fn(I1(), I16(), odd)
+        : D <= 2048 ? fn(Chunks(), W4(), odd)
+        : D <= 4096 ? fn(Chunks(), W8(), odd)
+        : D <= 8192 ? fn(Chunks(), W16(), odd)
                     : fn(I2(), I16(), odd);
   };
   return D % kChunk ? go(std::true_type()) : go(std::false_type());
@@ -759,7 +801,7 @@ hipError_t norm_fwd_t(
     return hipGetLastError();
   }
   // 8 waves a SIMD: 2048 blocks of 256 threads, 512 of 1024
-  return by_width(D, [&](auto nch, auto waves, auto odd) {
+  return by_width<true>(D, [&](auto nch, auto waves, auto odd) {
     constexpr int W = decltype(waves)::value;
     constexpr int threads = W == 1 ? 256 : W * kWave;
     const long need = W == 1 ? (R + 3) / 4 : R;
@@ -802,7 +844,7 @@ hipError_t norm_bwd_t(
       KFAC_HIP_CHECK(hipGetLastError());
     }
   } else {
-    KFAC_HIP_CHECK(by_width(D, [&](auto nch, auto waves, auto odd) {
+    KFAC_HIP_CHECK(by_width<false>(D, [&](auto nch, auto waves, auto odd) {
       constexpr int N = decltype(nch)::value, W = decltype(waves)::value;
       constexpr bool ODD = decltype(odd)::value;
       if (x != nullptr) {

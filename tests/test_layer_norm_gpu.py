@@ -20,7 +20,8 @@ PAIRS = [
 # around the widths where a row takes more lanes, and beyond registers
 WIDTHS = [
     1, 2, 7, 8, 9, 15, 63, 65, 71, 129, 256, 511, 512, 513, 768, 1001, 1024, 1025, 2047,
-    2048, 2049, 4096, 4097, 8192, 8193, 16384, 16385, 20001, 33000,
+    2048, 2049, 2304, 3001, 4095, 4096, 4097, 4160, 6001, 8191, 8192, 8193, 12001, 16384,
+    16385, 20001, 33000,
 ]
 
 
