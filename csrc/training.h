@@ -55,7 +55,7 @@ hipError_t norm_bwd_t(
 
 // How a weight gradient is cut into blocks.
 struct WGradPlan {
-  bool large;            // tiles
+  int tiles;             // small, large or narrow ones
   int splits;            // of the tokens
   int tiles_n, tiles_k;  // of the output
   int bias_tiles;        // of a row, which share the bias's sum

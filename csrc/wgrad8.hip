@@ -70,10 +70,12 @@ __device__ __forceinline__ Tile tile_of(const WGrad& a) {
 }
 
 // 16 byte chunk c of row r: the 64 byte group is swapped by the row, so
-// that the four rows of a transposed read lie in different banks.
+// that the four rows of a transposed read lie in different banks. Four rows
+// of 32 columns are the 64 banks as they are.
 template <int WIDTH>
 __device__ __forceinline__ int slot(int r, int c) {
-  return r * (WIDTH / 8) + (c ^ ((r & 3) << 2));
+  static_assert(WIDTH == 32 || WIDTH >= 128, "");
+  return r * (WIDTH / 8) + (WIDTH == 32 ? c : c ^ ((r & 3) << 2));
 }
 
 // Where a lane's part of the fragment of 32 columns starts: its 8 tokens are
@@ -121,12 +123,13 @@ __global__ __launch_bounds__(WN * WK * kWave) void wgrad8_kernel(WGrad a) {
   constexpr int kT = WN * WK * kWave;
   constexpr int TN = BN / WN, TK = BK / WK;        // a wave's part
   constexpr int FN = TN / 32, FK = TK / 32;        // in fragments
-  constexpr int GC = BM * BN / 8 / kT;             // chunks a thread, g
+  constexpr int kG = BM * BN / 8 < kT ? BM * BN / 8 : kT;
+  constexpr int GC = BM * BN / 8 / kG;             // chunks a thread, g
   constexpr int XC = BM * BK / 16 / kT;            // 16 codes each
   constexpr int kImage = BM * (NP * BN + BK);      // of one stage
   constexpr int kSteps = BM / 16;
-  static_assert(GC * kT * 8 == BM * BN && XC * kT * 16 == BM * BK, "");
-  static_assert(kT % (BN / 8) == 0, "a thread keeps its columns");
+  static_assert(GC * kG * 8 == BM * BN && XC * kT * 16 == BM * BK, "");
+  static_assert(kG % (BN / 8) == 0, "a thread keeps its columns");
   __shared__ __attribute__((aligned(16))) short lds[2 * kImage];
 
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
@@ -153,11 +156,12 @@ __global__ __launch_bounds__(WN * WK * kWave) void wgrad8_kernel(WGrad a) {
   }
   float bias[8] = {};
 
-  // This thread's pieces of a stage: chunk i of g is kT / (BN / 8) rows
-  // below chunk i - 1, and so on.
-  const int g_row = tid / (BN / 8), g_col = tid % (BN / 8) * 8;
+  // This thread's pieces of a stage: chunk i of g is kG / (BN / 8) rows
+  // below chunk i - 1, and so on. Where g has fewer chunks than there are
+  // threads, those behind kG do what the first ones do.
+  const int g_row = tid % kG / (BN / 8), g_col = tid % (BN / 8) * 8;
   const int x_row = tid / (BK / 16), x_col = tid % (BK / 16) * 16;
-  constexpr int kGDown = kT / (BN / 8), kXDown = kT / (BK / 16);
+  constexpr int kGDown = kG / (BN / 8), kXDown = kT / (BK / 16);
   // Offsets that differ from lane to lane, next to addresses that do not.
   // A chunk right of the matrix reads the tile's first one instead.
   const int gc = n0 + g_col < a.N ? g_col : 0;
@@ -397,7 +401,9 @@ __global__ __launch_bounds__(WN * WK * kWave) void wgrad8_kernel(WGrad a) {
     float* part = (float*)lds;
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 8; ++j) part[g_row * BN + g_col + j] = bias[j];
+    for (int j = 0; j < 8; ++j) {
+      if (tid < kG) part[g_row * BN + g_col + j] = bias[j];
+    }
     __syncthreads();
     for (int c = tid; c < BN; c += kT) {
       float s = 0.f;
@@ -492,17 +498,22 @@ template <typename TG>
 constexpr int kParts =
     sizeof(TG) == 4 ? 3 : std::is_same<TG, __half>::value ? 2 : 1;
 
-// The tiles of a product, large and small. Two images are 128 KB of LDS for
-// large bf16 tiles, one block to a compute unit, and 80 KB or less for the
-// others, two blocks.
-template <typename TG, bool LARGE>
+// The tiles of a product: small, large, and for up to 32 outputs narrow ones.
+// Two images are 128 KB of LDS for large bf16 tiles, one block to a compute
+// unit, and 80 KB or less for the others, two blocks or three.
+enum Tiles { kSmall, kLarge, kNarrow };
+
+template <typename TG, int TILES>
 struct Cut {
   static constexpr int NP = kParts<TG>;
-  static constexpr int BN = LARGE && NP == 1 ? 256 : 128;
-  static constexpr int BK = LARGE ? 256 : 128;
+  static constexpr int BN =
+      TILES == kNarrow ? 32 : TILES == kLarge && NP == 1 ? 256 : 128;
+  static constexpr int BK = TILES == kSmall ? 128 : 256;
   static constexpr int BM = NP == 1 ? 64 : 32;
-  static constexpr int WN = 2, WK = LARGE ? 4 : 2;
-  static constexpr int kSlots = LARGE && NP == 1 ? 1 : 2;
+  static constexpr int WN = TILES == kNarrow ? 1 : 2;
+  static constexpr int WK = TILES == kSmall ? 2 : 4;
+  static constexpr int kSlots =
+      TILES == kNarrow && NP > 1 ? 3 : TILES == kLarge && NP == 1 ? 1 : 2;
 };
 
 // What a call takes, in us, by a model with the numbers of 40 shapes on
@@ -511,9 +522,12 @@ struct Cut {
 // a block takes 8 to 10 us beside its stages, a stage the longer the fuller
 // the compute unit. Small tiles need more reads for each product (a stage
 // of a quarter of the area takes 1.2 us for two blocks, not 0.95), but
-// leave less to be added where the tokens are split.
+// leave less to be added where the tokens are split. Narrow tiles multiply no
+// padding where there are few outputs (16384 x 32 x 4096: bf16 25 us, 30 with
+// small tiles; fp32 32 us, 61; 64 outputs fp32 48 us, 72; of 96 nothing is
+// gained). Few inputs gain little, since a wide gradient is what is read.
 struct Rates {
-  float alone[2], full[2];  // a stage with half a card's blocks and with all
+  float alone[3], full[3];  // a stage with half a card's blocks and with all
   float block;
   float add;       // a second launch
   float per_byte;  // of the splits' sums, written and read
@@ -522,21 +536,21 @@ struct Rates {
 
 template <typename TG>
 constexpr Rates kRates = kParts<TG> == 1
-    ? Rates{{0.73f, 1.65f}, {1.22f, 1.89f}, 10.4f, 2.8f, 1.05e-7f, 0.06f}
+    ? Rates{{0.73f, 1.65f, 0.8f}, {1.22f, 1.89f, 1.6f}, 10.4f, 2.8f, 1.05e-7f, 0.06f}
     : kParts<TG> == 2
-    ? Rates{{0.67f, 0.83f}, {1.00f, 2.14f}, 8.1f, 3.8f, 1.37e-7f, 0.06f}
-    : Rates{{0.91f, 1.17f}, {1.55f, 3.09f}, 8.6f, 3.2f, 1.36e-7f, 0.07f};
+    ? Rates{{0.67f, 0.83f, 0.55f}, {1.00f, 2.14f, 1.2f}, 8.1f, 3.8f, 1.37e-7f, 0.06f}
+    : Rates{{0.91f, 1.17f, 0.9f}, {1.55f, 3.09f, 1.76f}, 8.6f, 3.2f, 1.36e-7f, 0.07f};
 
-template <typename TG, bool LARGE>
+template <typename TG, int TILES>
 void consider(long M, int N, int K, WGradPlan& best, float& best_time) {
-  using C = Cut<TG, LARGE>;
+  using C = Cut<TG, TILES>;
   constexpr Rates rates = kRates<TG>;
   constexpr int kSlots = 256 * C::kSlots;
   const long tiles_n = ceil_div(N, C::BN), tiles_k = ceil_div(K, C::BK);
   const long tiles = tiles_n * tiles_k;
   const long stages = (M + C::BM - 1) / C::BM;
   long last = 0;
-  for (const int blocks : {0, 64, 128, 192, 256, 384, 512}) {
+  for (const int blocks : {0, 64, 128, 192, 256, 384, 512, 768}) {
     long s = (blocks + tiles / 2) / tiles;
     s = s < 1 ? 1 : s > stages ? stages : s;
     const long per = (stages + s - 1) / s;
@@ -545,15 +559,15 @@ void consider(long M, int N, int K, WGradPlan& best, float& best_time) {
     last = s;
     const long all = s * tiles, left = all % kSlots;
     float time = (float)(all / kSlots) *
-        (rates.block + (float)per * rates.full[LARGE]);
+        (rates.block + (float)per * rates.full[TILES]);
     if (left > 0) {
       // from half a block for each compute unit to all of its blocks
       float load = ((float)left / 256.f - 0.5f) / (C::kSlots - 0.5f);
       load = load < 0.f ? 0.f : load;
       time += rates.block +
           (float)per *
-              (rates.alone[LARGE] +
-               load * (rates.full[LARGE] - rates.alone[LARGE]));
+              (rates.alone[TILES] +
+               load * (rates.full[TILES] - rates.alone[TILES]));
     }
     if (s > 1) {
       time += rates.add + (float)s * rates.per_row +
@@ -565,7 +579,7 @@ void consider(long M, int N, int K, WGradPlan& best, float& best_time) {
       // launch: some 10 % of its stages against 2.5 us.
       const bool alone = s == 1 && per <= 16;
       const long share = alone ? 1 : per < tiles_k ? per : tiles_k;
-      best = {LARGE, (int)s, (int)tiles_n, (int)tiles_k, (int)share,
+      best = {TILES, (int)s, (int)tiles_n, (int)tiles_k, (int)share,
               per * C::BM};
     }
   }
@@ -575,8 +589,9 @@ template <typename TG>
 WGradPlan wgrad8_plan(long M, int N, int K) {
   WGradPlan best{};
   float time = __builtin_inff();
-  consider<TG, false>(M, N, K, best, time);
-  consider<TG, true>(M, N, K, best, time);
+  consider<TG, kSmall>(M, N, K, best, time);
+  consider<TG, kLarge>(M, N, K, best, time);
+  if (N <= 64) consider<TG, kNarrow>(M, N, K, best, time);
   return best;
 }
 
@@ -595,13 +610,15 @@ hipError_t wgrad8_t(
   WGrad a{g,    codes, exps, sums, bias, M, N, K, ceil_div(K, kBlock8),
           plan.tiles_n, plan.tiles_k, plan.bias_tiles, plan.rows};
   const unsigned grid = (unsigned)plan.splits * plan.tiles_n * plan.tiles_k;
-  const auto go = [&](auto large) {
-    using C = Cut<TG, decltype(large)::value>;
+  const auto go = [&](auto tiles) {
+    using C = Cut<TG, decltype(tiles)::value>;
     wgrad8_kernel<TG, C::NP, C::BN, C::BK, C::BM, C::WN, C::WK>
         <<<grid, C::WN * C::WK * kWave, 0, s>>>(a);
     return hipGetLastError();
   };
-  return plan.large ? go(std::true_type()) : go(std::false_type());
+  return plan.tiles == kSmall ? go(std::integral_constant<int, kSmall>())
+      : plan.tiles == kLarge  ? go(std::integral_constant<int, kLarge>())
+                              : go(std::integral_constant<int, kNarrow>());
 }
 
 hipError_t wgrad8_add(

@@ -132,7 +132,8 @@ def test_gelu8_every_sixteen_bit_value(dtype, approximate) -> None:
         (1, 1, 1), (1, 5, 64), (2, 128, 128), (31, 33, 65), (64, 256, 256),
         (65, 129, 127), (200, 8, 1000), (1000, 517, 8), (1280, 256, 256),
         (4099, 300, 200), (777, 1001, 333), (3000, 768, 768),
-        (33, 2304, 768), (20000, 16, 16),
+        (33, 2304, 768), (20000, 16, 16), (5000, 32, 4096), (3001, 12, 3415),
+        (700, 33, 1025), (9, 64, 6144), (4097, 1, 2000), (16384, 63, 519),
     ],
 )
 def test_weight_grad8(dtype, m, n, k) -> None:
