@@ -132,7 +132,8 @@ __global__ __launch_bounds__(WN * WK * kWave) void wgrad8_kernel(WGrad a) {
   static_assert(kG % (BN / 8) == 0, "a thread keeps its columns");
   __shared__ __attribute__((aligned(16))) short lds[2 * kImage];
 
-  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const int tid = threadIdx.x, lane = tid % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const Tile tile = tile_of(a);
   const int n0 = tile.n * BN, k0 = tile.k * BK;
   const long m0 = tile.split * a.rows;
@@ -384,15 +385,33 @@ __global__ __launch_bounds__(WN * WK * kWave) void wgrad8_kernel(WGrad a) {
 
   // column lane % 32, rows 8 * (r / 4) + 4 * (lane / 32) + r % 4
   float* out = a.out + (long)tile.split * a.N * a.K;
+  if (n0 + BN <= a.N && k0 + BK <= a.K) {
+    // A row's address is the same for a wave: 3 operations a store, not 10
+    // (0.8 us of 128 x 128 values, not 1.8).
+    float* first = out + (long)(n0 + wn) * a.K + k0 + wk;
+    const unsigned at = (unsigned)(lane / 32 * 4) * a.K + lane % 32;
 #pragma unroll
-  for (int i = 0; i < FN; ++i) {
+    for (int i = 0; i < FN; ++i) {
 #pragma unroll
-    for (int j = 0; j < FK; ++j) {
-      const int k = k0 + wk + j * 32 + lane % 32;
+      for (int j = 0; j < FK; ++j) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int n = n0 + wn + i * 32 + r / 4 * 8 + lane / 32 * 4 + r % 4;
-        if (n < a.N && k < a.K) out[(long)n * a.K + k] = acc[i][j][r];
+        for (int r = 0; r < 16; ++r) {
+          const int n = i * 32 + r / 4 * 8 + r % 4;
+          *lane_ptr(first + (long)n * a.K + j * 32, at) = acc[i][j][r];
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < FN; ++i) {
+#pragma unroll
+      for (int j = 0; j < FK; ++j) {
+        const int k = k0 + wk + j * 32 + lane % 32;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int n = n0 + wn + i * 32 + r / 4 * 8 + lane / 32 * 4 + r % 4;
+          if (n < a.N && k < a.K) out[(long)n * a.K + k] = acc[i][j][r];
+        }
       }
     }
   }
