@@ -19,11 +19,11 @@
 // fill the card; the splits' fp32 sums are added by a second kernel in a
 // fixed order.
 //
-// Measured: 16384 tokens x 8192 x 4096 bf16 899 us (1223 TFLOP/s; a product
+// Measured: 16384 tokens x 8192 x 4096 bf16 894 us (1230 TFLOP/s; a product
 // of 8192^3 by the library 1228), bound by the clock that the power limit
-// leaves; 16384 x 768 x 2304 76 us: 65 in the products, 14 of them to start,
-// end and write 9 splits' sums, and 12 to add these; 8192 x 4096 x 4096 fp32
-// 720 us (382 TFLOP/s, three times that on the matrix cores).
+// leaves; 16384 x 768 x 2304 73 us: 50 in the products, 13 to start, end and
+// write 9 splits' sums, and 12 to add these; 8192 x 4096 x 4096 fp32 700 us
+// (393 TFLOP/s, three times that on the matrix cores).
 
 #include "act8.h"
 
