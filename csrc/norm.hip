@@ -10,8 +10,9 @@
 //
 // Both passes are bound by memory, so a row is read once: it stays in
 // registers between its sums and its outputs, 8 values a lane and chunk,
-// one wave a row up to 1024 values, 4, 8 or 16 up to 2048, 4096 or 16384 (the
-// forward pass by half for lengths that are no multiple of 8). The
+// 8, 16 or 32 lanes a row up to 64, 128 or 256 values, one wave up to 1024, 4,
+// 8 or 16 up to 2048, 4096 or 16384 (the forward pass by half for lengths that
+// are no multiple of 8). The
 // variance is the mean of the centred squares of those registers, never a
 // difference of two large sums. The backward pass keeps dw and db of its
 // rows in registers too and writes one partial row a block; a second kernel
@@ -36,28 +37,49 @@ __device__ __forceinline__ float add_dpp(float v) {
                  __float_as_int(v), CTRL, 0xf, 0xf, true));
 }
 
-// Sum over a wave, the same bits in each lane: quads, halves and rows of 16
-// by register permutations, rows and halves of the wave by swaps.
-__device__ __forceinline__ float wave_sum(float v) {
-  v = add_dpp<0xB1>(v);
-  v = add_dpp<0x4E>(v);
-  v = add_dpp<0x141>(v);
-  v = add_dpp<0x140>(v);
+// v of the lane and of the one 16 (32) further, round the wave
+__device__ __forceinline__ float add_swap16(float v) {
   const unsigned u = __float_as_uint(v);
   const auto row = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-  v = __uint_as_float(row[0]) + __uint_as_float(row[1]);
-  const unsigned w = __float_as_uint(v);
-  const auto half = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return __uint_as_float(row[0]) + __uint_as_float(row[1]);
+}
+__device__ __forceinline__ float add_swap32(float v) {
+  const unsigned u = __float_as_uint(v);
+  const auto half = __builtin_amdgcn_permlane32_swap(u, u, false, false);
   return __uint_as_float(half[0]) + __uint_as_float(half[1]);
 }
 
-// Sum over the W waves of a row; every wave of the block calls it, as often
-// as the others. `at` alternates between two halves of `lds`, so that one
-// barrier a sum is enough.
-template <int W>
+// Sum over each 8, 16, 32 or 64 lanes, the same bits in all of them: quads,
+// halves and rows of 16 by register permutations, rows and halves of the
+// wave by swaps.
+template <int LANES>
+__device__ __forceinline__ float lane_sum(float v) {
+  v = add_dpp<0xB1>(v);
+  v = add_dpp<0x4E>(v);
+  v = add_dpp<0x141>(v);
+  if (LANES >= 16) v = add_dpp<0x140>(v);
+  if (LANES >= 32) v = add_swap16(v);
+  if (LANES >= 64) v = add_swap32(v);
+  return v;
+}
+
+// Sum over the lanes of a wave that are LANES, 2 * LANES ... apart.
+template <int LANES>
+__device__ __forceinline__ float sum_across(float v) {
+  if (LANES <= 8) v = add_dpp<0x128>(v);  // a row of 16 turned by 8
+  if (LANES <= 16) v = add_swap16(v);
+  if (LANES <= 32) v = add_swap32(v);
+  return v;
+}
+
+// Sum over the LANES of a row: part of a wave, or several waves, whose blocks
+// call it with all of them, as often as each other. `at` alternates between
+// two halves of `lds`, so that one barrier a sum is enough.
+template <int LANES>
 __device__ __forceinline__ float row_sum(float v, float* lds, int& at) {
-  v = wave_sum(v);
-  if (W == 1) return v;
+  constexpr int W = LANES / kWave;
+  v = lane_sum<W == 0 ? LANES : kWave>(v);
+  if (W <= 1) return v;
   const int wave = threadIdx.x / kWave;
   float* slot = lds + at * 16;
   at ^= 1;
@@ -117,10 +139,28 @@ struct Forward {
   float eps;
 };
 
-// A wave's row number, in a scalar register: rows are the same for a wave's
-// lanes, and addresses then cost no vector registers.
-__device__ __forceinline__ int group_of(int threads) {
-  return __builtin_amdgcn_readfirstlane(threadIdx.x / threads);
+// Rows of up to 64, 128 and 256 values take 8, 16 and 32 lanes, so that a
+// wave has 8, 4 or 2 of them: rows_of_wave. Its first row's number is in a
+// scalar register (wide rows have one for each of their waves), and addresses
+// cost no vector registers: the others are some 32 bit offset further down.
+// Where there are no more rows, lanes repeat the first one, to the bit. These
+// kernels are bound by arithmetic where lanes are idle: 196608 rows of 64 bf16
+// values take 10 us forward and 17 backward, 51 and 56 with a wave a row.
+constexpr int rows_of_wave(int lanes) {
+  return lanes < kWave ? kWave / lanes : 1;
+}
+template <int LANES>
+__device__ __forceinline__ int group_of() {
+  constexpr int threads = LANES < kWave ? kWave : LANES;
+  return __builtin_amdgcn_readfirstlane(threadIdx.x / threads) *
+      rows_of_wave(LANES);
+}
+// The lane's row, counted from the wave's first, of which there are `left`.
+template <int LANES>
+__device__ __forceinline__ int down_of(long left) {
+  if (LANES >= kWave) return 0;
+  const int down = threadIdx.x % kWave / LANES;
+  return down < left ? down : 0;
 }
 
 // The part of a row that a lane holds in chunk i of its NCH: 8 values from
@@ -131,12 +171,13 @@ __device__ __forceinline__ int group_of(int threads) {
 struct Part {
   int chunk;
   unsigned col;
+  unsigned at;  // the column, from the start of the wave's first row
   int skip;
   bool any;
 };
 
 template <bool ODD, int LANES, int NCH>
-__device__ __forceinline__ Part part_of(int lane, int i, int D) {
+__device__ __forceinline__ Part part_of(int lane, int i, int D, int down = 0) {
   Part p;
   p.chunk = lane + i * LANES;
   const int col = p.chunk * kChunk;
@@ -145,18 +186,20 @@ __device__ __forceinline__ Part part_of(int lane, int i, int D) {
   p.any = whole || col < D;
   p.skip = ODD && !whole && p.any && col > D - kChunk ? col - (D - kChunk) : 0;
   p.col = p.any ? col - p.skip : 0;
+  p.at = down * D + p.col;
   return p;
 }
 
-// How many of the kSpan columns that a wave's last chunks cover are in the
-// row: kSpan or more if all are, 0 or less if the wave is right of its end.
-constexpr int kSpan = kWave * kChunk;
-
-template <int W, int NCH>
+// How many of the columns that a wave's last chunks of a row cover are in it:
+// span_of or more if all are, 0 or less if the wave is right of its end.
+constexpr int span_of(int lanes) {
+  return (lanes < kWave ? lanes : kWave) * kChunk;
+}
+template <int LANES, int NCH>
 __device__ __forceinline__ int columns_of(int D) {
   const int wave =
-      W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  return D - ((NCH - 1) * W + wave) * kSpan;
+      LANES <= kWave ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  return D - (NCH - 1) * LANES * kChunk - wave * kWave * kChunk;
 }
 
 // The lane's number, new to the compiler in each turn of a loop: it would
@@ -166,53 +209,54 @@ __device__ __forceinline__ int fresh(int lane) {
   return lane;
 }
 
-template <typename TX, typename TY, int NCH, int W, bool ODD>
-__global__ __launch_bounds__(W == 1 ? 256 : W * kWave) void norm_fwd_kernel(
+template <typename TX, typename TY, int NCH, int LANES, bool ODD>
+__global__ __launch_bounds__(
+    LANES <= kWave ? 256 : LANES) void norm_fwd_kernel(
     Forward<TX, TY> a) {
-  constexpr int kLanes = W * kWave;
-  constexpr int G = W == 1 ? 4 : 1;  // rows of a block
+  constexpr int G = LANES <= kWave ? 4 * rows_of_wave(LANES) : 1;  // of a block
   __shared__ float lds[32];
   int at = 0;
-  const int lane0 = threadIdx.x % kLanes;
-  const int group = group_of(kLanes);
+  const int lane0 = threadIdx.x % LANES;
+  const int group = group_of<LANES>();
   float w[NCH][8], b[NCH][8];
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
-    const Part p = part_of<ODD, kLanes, NCH>(lane0, i, a.D);
+    const Part p = part_of<ODD, LANES, NCH>(lane0, i, a.D);
 #pragma unroll
     for (int j = 0; j < kChunk; ++j) w[i][j] = 1.f, b[i][j] = 0.f;
     if (a.w.p != nullptr) load_any(a.w, 0, p.col, w[i]);
     if (a.b.p != nullptr) load_any(a.b, 0, p.col, b[i]);
   }
-  const int columns = columns_of<W, NCH>(a.D);
+  const int columns = columns_of<LANES, NCH>(a.D);
   for (long base = (long)blockIdx.x * G; base < a.R;
        base += (long)gridDim.x * G) {
     const long row = base + group;
-    if (W == 1 && row >= a.R) return;
-    if (NCH == 1 && W > 1 && columns <= 0) {
+    if (LANES <= kWave && row >= a.R) return;
+    if (NCH == 1 && LANES > kWave && columns <= 0) {
       // right of the row's end: only keeps the others company
-      row_sum<W>(0.f, lds, at);
-      row_sum<W>(0.f, lds, at);
+      row_sum<LANES>(0.f, lds, at);
+      row_sum<LANES>(0.f, lds, at);
       continue;
     }
     const long start = row * a.D;
     const int lane = fresh(lane0);
+    const int down = down_of<LANES>(a.R - row);
     float t[NCH][8];
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const Part p = part_of<ODD, kLanes, NCH>(lane, i, a.D);
-      load8(lane_ptr(a.x + start, p.col), t[i]);
+      const Part p = part_of<ODD, LANES, NCH>(lane, i, a.D, down);
+      load8(lane_ptr(a.x + start, p.at), t[i]);
       if (a.r.p != nullptr) {
         float r[8];
-        load_any(a.r, start, p.col, r);
+        load_any(a.r, start, p.at, r);
 #pragma unroll
         for (int j = 0; j < kChunk; ++j) {
           t[i][j] = round_to(t[i][j] + r[j], a.x);
         }
-        if (p.any) store8(lane_ptr(a.total + start, p.col), t[i]);
+        if (p.any) store8(lane_ptr(a.total + start, p.at), t[i]);
       }
-      if (i + 1 < NCH || columns >= kSpan) {
+      if (i + 1 < NCH || columns >= span_of(LANES)) {
 #pragma unroll
         for (int j = 0; j < kChunk; ++j) sum += t[i][j];
       } else {
@@ -222,12 +266,12 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * kWave) void norm_fwd_kernel(
         }
       }
     }
-    const float mean = row_sum<W>(sum, lds, at) / a.D;
+    const float mean = row_sum<LANES>(sum, lds, at) / a.D;
     float square = 0.f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const Part p = part_of<ODD, kLanes, NCH>(lane, i, a.D);
-      if (i + 1 < NCH || columns >= kSpan) {
+      const Part p = part_of<ODD, LANES, NCH>(lane, i, a.D, down);
+      if (i + 1 < NCH || columns >= span_of(LANES)) {
 #pragma unroll
         for (int j = 0; j < kChunk; ++j) {
           const float c = t[i][j] - mean;
@@ -241,31 +285,31 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * kWave) void norm_fwd_kernel(
         }
       }
     }
-    const float var = row_sum<W>(square, lds, at) / a.D;
+    const float var = row_sum<LANES>(square, lds, at) / a.D;
     const float rstd = reciprocal_root(var + a.eps);
     if (lane == 0) {
-      a.mean[row] = mean;
-      a.rstd[row] = rstd;
+      (a.mean + row)[down] = mean;
+      (a.rstd + row)[down] = rstd;
     }
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const Part p = part_of<ODD, kLanes, NCH>(lane, i, a.D);
+      const Part p = part_of<ODD, LANES, NCH>(lane, i, a.D, down);
       const long block = row * a.blocks;
       if (a.in_codes != nullptr) {
         pack_chunk<ODD>(
-            t[i], p.any, p.skip, kChunk, lane_ptr(a.in_codes + start, p.col),
-            lane_ptr(a.in_exps + block, p.chunk / 8), p.chunk % 8 == 0);
+            t[i], p.any, p.skip, kChunk, lane_ptr(a.in_codes + start, p.at),
+            lane_ptr(a.in_exps + block, down * a.blocks + p.chunk / 8), p.chunk % 8 == 0);
       }
 #pragma unroll
       for (int j = 0; j < kChunk; ++j) {
         const float h = (t[i][j] - mean) * rstd;
         t[i][j] = round_to(h * w[i][j] + b[i][j], a.y);
       }
-      if (p.any) store8(lane_ptr(a.y + start, p.col), t[i]);
+      if (p.any) store8(lane_ptr(a.y + start, p.at), t[i]);
       if (a.out_codes != nullptr) {
         pack_chunk<ODD>(
-            t[i], p.any, p.skip, kChunk, lane_ptr(a.out_codes + start, p.col),
-            lane_ptr(a.out_exps + block, p.chunk / 8), p.chunk % 8 == 0);
+            t[i], p.any, p.skip, kChunk, lane_ptr(a.out_codes + start, p.at),
+            lane_ptr(a.out_exps + block, down * a.blocks + p.chunk / 8), p.chunk % 8 == 0);
       }
     }
   }
@@ -323,25 +367,28 @@ struct KeptRow {
   __device__ __forceinline__ void fetch(
       const Backward<TX, TY>& a,
       long row,
-      int lane) {
+      int lane,
+      int down) {
     const long start = row * a.D;
-    mean = a.mean[row];
-    rstd = a.rstd[row];
+    mean = (a.mean + row)[down];
+    rstd = (a.rstd + row)[down];
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const Part p = part_of<ODD, LANES, NCH>(lane, i, a.D);
-      dy[i].load(lane_ptr(a.dy + start, p.col));
+      const Part p = part_of<ODD, LANES, NCH>(lane, i, a.D, down);
+      dy[i].load(lane_ptr(a.dy + start, p.at));
       if (KEPT8) {
         const uint8_t* e = a.exps + row * a.blocks;
-        byte[i] = *lane_ptr(e, p.col / kBlock8);
+        byte[i] = *lane_ptr(e, down * a.blocks + p.col / kBlock8);
         // the last lane's own values may be in the next block
-        if (ODD) own[i] = *lane_ptr(e, p.any ? p.chunk / 8 : 0);
+        if (ODD) {
+          own[i] = *lane_ptr(e, down * a.blocks + (p.any ? p.chunk / 8 : 0));
+        }
         unsigned c[2];
-        __builtin_memcpy(c, lane_ptr(a.codes + start, p.col), 8);
+        __builtin_memcpy(c, lane_ptr(a.codes + start, p.at), 8);
         x[i].v[0][0] = c[0];
         x[i].v[0][1] = c[1];
       } else {
-        x[i].load(lane_ptr(a.x + start, p.col));
+        x[i].load(lane_ptr(a.x + start, p.at));
       }
     }
   }
@@ -366,22 +413,22 @@ struct KeptRow {
   }
 };
 
-template <typename TX, typename TY, int NCH, int W, bool ODD, bool KEPT8>
+template <typename TX, typename TY, int NCH, int LANES, bool ODD, bool KEPT8>
 __global__ __launch_bounds__(1024) void norm_bwd_kernel(Backward<TX, TY> a) {
-  constexpr int kLanes = W * kWave;
-  constexpr int G = 16 / W;                     // rows of a block
-  constexpr int kAll = kLanes * kChunk * NCH;   // columns of a group
+  constexpr int S = rows_of_wave(LANES);
+  constexpr int G = LANES < kWave ? 16 : 1024 / LANES;  // groups of a block
+  constexpr int kAll = LANES * kChunk * NCH;            // columns of a group
   __shared__ float lds[32];
   __shared__ __attribute__((aligned(16))) float
       parts[G > 1 ? 2 * G * kAll : 4];
   int at = 0;
-  const int lane0 = threadIdx.x % kLanes;
-  const int group = group_of(kLanes);
+  const int lane0 = threadIdx.x % LANES;
+  const int group = group_of<LANES>();  // its first row
   const float mean_of = 1.f / a.D;
   float w[NCH][8], dw[NCH][8], db[NCH][8];
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
-    const Part p = part_of<ODD, kLanes, NCH>(lane0, i, a.D);
+    const Part p = part_of<ODD, LANES, NCH>(lane0, i, a.D);
 #pragma unroll
     for (int j = 0; j < kChunk; ++j) {
       w[i][j] = 1.f;
@@ -393,21 +440,24 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(Backward<TX, TY> a) {
   // row's loads have to be under way before the last row is done with (16384
   // x 8192 bf16: 176 us without, 159 us with it, 5.1 TB/s). Single waves wait
   // for their rows in their own time.
-  constexpr bool kAhead = W > 1 && NCH == 1;  // two chunks would spill
+  constexpr bool kAhead = LANES > kWave && NCH == 1;  // two chunks would spill
   KeptRow<TX, TY, NCH> next;
   if (kAhead) {
     const long row = (long)blockIdx.x * G + group;
-    next.template fetch<ODD, KEPT8, kLanes>(a, row < a.R ? row : 0, lane0);
+    next.template fetch<ODD, KEPT8, LANES>(a, row < a.R ? row : 0, lane0, 0);
   }
-  for (long base = (long)blockIdx.x * G; base < a.R;
-       base += (long)gridDim.x * G) {
-    const bool live = base + group < a.R;
-    if (W == 1 && !live) break;
+  for (long base = (long)blockIdx.x * G * S; base < a.R;
+       base += (long)gridDim.x * G * S) {
+    const bool some = base + group < a.R;
+    if (LANES <= kWave && !some) break;
     // a group without a row takes part in the barriers, with row 0
-    const long row = live ? base + group : 0;
+    const long row = some ? base + group : 0;
     const long start = row * a.D;
     const int lane = fresh(lane0);
-    if (!kAhead) next.template fetch<ODD, KEPT8, kLanes>(a, row, lane);
+    const int down = down_of<LANES>(a.R - row);
+    const bool live =
+        some && (S == 1 || row + (int)threadIdx.x % kWave / LANES < a.R);
+    if (!kAhead) next.template fetch<ODD, KEPT8, LANES>(a, row, lane, down);
     const float mean = next.mean, rstd = next.rstd;
     Raw<TY> dy[NCH];
     Raw<TX> dt[NCH];
@@ -415,15 +465,15 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(Backward<TX, TY> a) {
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const Part p = part_of<ODD, kLanes, NCH>(lane, i, a.D);
+      const Part p = part_of<ODD, LANES, NCH>(lane, i, a.D, down);
       dy[i] = next.dy[i];
       next.template values<ODD, KEPT8>(i, p, h[i]);
     }
     if (a.dt != nullptr) {
 #pragma unroll
       for (int i = 0; i < NCH; ++i) {
-        const Part p = part_of<ODD, kLanes, NCH>(lane, i, a.D);
-        dt[i].load(lane_ptr(a.dt + start, p.col));
+        const Part p = part_of<ODD, LANES, NCH>(lane, i, a.D, down);
+        dt[i].load(lane_ptr(a.dt + start, p.at));
       }
     } else {
 #pragma unroll
@@ -431,12 +481,12 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(Backward<TX, TY> a) {
     }
     if (kAhead) {
       const long then = base + (long)gridDim.x * G + group;
-      next.template fetch<ODD, KEPT8, kLanes>(
-          a, then < a.R ? then : 0, lane);
+      next.template fetch<ODD, KEPT8, LANES>(
+          a, then < a.R ? then : 0, lane, 0);
     }
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const Part p = part_of<ODD, kLanes, NCH>(lane, i, a.D);
+      const Part p = part_of<ODD, LANES, NCH>(lane, i, a.D, down);
       float g[8];
       dy[i].values(g);
 #pragma unroll
@@ -452,11 +502,11 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(Backward<TX, TY> a) {
         s2 += product * w[i][j];
       }
     }
-    s1 = row_sum<W>(s1, lds, at) * mean_of;
-    s2 = row_sum<W>(s2, lds, at) * mean_of;
+    s1 = row_sum<LANES>(s1, lds, at) * mean_of;
+    s2 = row_sum<LANES>(s2, lds, at) * mean_of;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const Part p = part_of<ODD, kLanes, NCH>(lane, i, a.D);
+      const Part p = part_of<ODD, LANES, NCH>(lane, i, a.D, down);
       float g[8], d[8];
       dy[i].values(g);
       dt[i].values(d);
@@ -464,7 +514,15 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(Backward<TX, TY> a) {
       for (int j = 0; j < kChunk; ++j) {
         d[j] += rstd * (g[j] * w[i][j] - s1 - h[i][j] * s2);
       }
-      if (live && p.any) store8(lane_ptr(a.dx + start, p.col), d);
+      if (live && p.any) store8(lane_ptr(a.dx + start, p.at), d);
+    }
+  }
+  // the rows of a wave, in the order of their lanes' permutations
+  if (S > 1) {
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) {
+      dw[0][j] = sum_across<LANES>(dw[0][j]);
+      db[0][j] = sum_across<LANES>(db[0][j]);
     }
   }
   // a single block's sums are the gradients
@@ -483,7 +541,7 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(Backward<TX, TY> a) {
     float* mine = a.partial + (long)blockIdx.x * 2 * a.D;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const Part p = part_of<ODD, kLanes, NCH>(lane0, i, a.D);
+      const Part p = part_of<ODD, LANES, NCH>(lane0, i, a.D);
       if (!p.any) continue;
       if (!single && p.skip == 0) {
         store8(mine + p.col, dw[i]);
@@ -505,7 +563,8 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(Backward<TX, TY> a) {
   const int last = ODD ? a.D / kChunk * kChunk : a.D;
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
-    float* mine = parts + group * kAll + (lane0 + i * kLanes) * kChunk;
+    float* mine = parts + group / S * kAll + (lane0 + i * LANES) * kChunk;
+    if (S > 1 && threadIdx.x % kWave >= LANES) continue;
     store8(mine, dw[i]);
     store8(mine + G * kAll, db[i]);
   }
@@ -586,7 +645,7 @@ __global__ __launch_bounds__(1024) void norm_fwd_long_kernel(
       for (int j = 0; j < kChunk; ++j) part += t[j];
       sum += part;
     }
-    const float mean = row_sum<16>(sum, lds, at) / a.D;
+    const float mean = row_sum<1024>(sum, lds, at) / a.D;
     float square = 0.f;
     for (int c0 = 0; c0 < a.D; c0 += kLongSpan) {
       const int col = c0 + first, n = a.D - col;
@@ -600,7 +659,7 @@ __global__ __launch_bounds__(1024) void norm_fwd_long_kernel(
       }
       square += part;
     }
-    const float var = row_sum<16>(square, lds, at) / a.D;
+    const float var = row_sum<1024>(square, lds, at) / a.D;
     const float rstd = reciprocal_root(var + a.eps);
     if (threadIdx.x == 0) {
       a.mean[row] = mean;
@@ -681,8 +740,8 @@ __global__ __launch_bounds__(1024) void norm_bwd_long_kernel(
         store_chunk(a.dx + start + col, n, q);
       }
       if (pass == 0) {
-        s1 = row_sum<16>(s1, lds, at) / a.D;
-        s2 = row_sum<16>(s2, lds, at) / a.D;
+        s1 = row_sum<1024>(s1, lds, at) / a.D;
+        s2 = row_sum<1024>(s2, lds, at) / a.D;
       }
     }
   }
@@ -722,7 +781,13 @@ unsigned long_blocks(long R) { return (unsigned)(R < 65536 ? R : 65536); }
 // Blocks of the backward kernel: what fills 256 compute units once, each
 // with the 16 waves that 128 registers a lane allow.
 int rows_of_block(int D) {
-  return D <= 1024 ? 16 : D <= 2048 ? 4 : D <= 4096 ? 2 : 1;
+  return D <= 64 ? 128
+      : D <= 128  ? 64
+      : D <= 256  ? 32
+      : D <= 1024 ? 16
+      : D <= 2048 ? 4
+      : D <= 4096 ? 2
+                  : 1;
 }
 
 // Calls fn with the kernel's template parameters (chunks of a lane, waves of
@@ -736,19 +801,20 @@ template <bool HALVED, typename Fn>
 hipError_t by_width(int D, Fn fn) {
   const auto go = [&](auto odd) {
     constexpr int kHalf = HALVED && decltype(odd)::value ? 2 : 1;
+    const auto call = [&](auto nch, auto lanes) { return fn(nch, lanes, odd); };
     using I1 = std::integral_constant<int, 1>;
     using I2 = std::integral_constant<int, 2>;
-    using I16 = std::integral_constant<int, 16>;
     using Chunks = std::integral_constant<int, kHalf>;
-    using W4 = std::integral_constant<int, 4 / kHalf>;
-    using W8 = std::integral_constant<int, 8 / kHalf>;
-    using W16 = std::integral_constant<int, 16 / kHalf>;
-    return D <= 512 ? fn(I1(), I1(), odd)
-        : D <= 1024 ? fn(I2(), I1(), odd)
-        : D <= 2048 ? fn(Chunks(), W4(), odd)
-        : D <= 4096 ? fn(Chunks(), W8(), odd)
-        : D <= 8192 ? fn(Chunks(), W16(), odd)
-                    : fn(I2(), I16(), odd);
+    return D <= 64  ? call(I1(), std::integral_constant<int, 8>())
+        : D <= 128  ? call(I1(), std::integral_constant<int, 16>())
+        : D <= 256  ? call(I1(), std::integral_constant<int, 32>())
+        : D <= 512  ? call(I1(), std::integral_constant<int, 64>())
+        : D <= 1024 ? call(I2(), std::integral_constant<int, 64>())
+        : D <= 2048 ? call(Chunks(), std::integral_constant<int, 256 / kHalf>())
+        : D <= 4096 ? call(Chunks(), std::integral_constant<int, 512 / kHalf>())
+        : D <= 8192
+        ? call(Chunks(), std::integral_constant<int, 1024 / kHalf>())
+        : call(I2(), std::integral_constant<int, 1024>());
   };
   return D % kChunk ? go(std::true_type()) : go(std::false_type());
 }
@@ -801,12 +867,13 @@ hipError_t norm_fwd_t(
     return hipGetLastError();
   }
   // 8 waves a SIMD: 2048 blocks of 256 threads, 512 of 1024
-  return by_width<true>(D, [&](auto nch, auto waves, auto odd) {
-    constexpr int W = decltype(waves)::value;
-    constexpr int threads = W == 1 ? 256 : W * kWave;
-    const long need = W == 1 ? (R + 3) / 4 : R;
+  return by_width<true>(D, [&](auto nch, auto lanes, auto odd) {
+    constexpr int N = decltype(nch)::value, L = decltype(lanes)::value;
+    constexpr int threads = L <= kWave ? 256 : L;
+    constexpr int rows = L <= kWave ? 4 * rows_of_wave(L) : 1;
+    const long need = (R + rows - 1) / rows;
     const long most = 2048L * 256 / threads;
-    norm_fwd_kernel<TX, TY, decltype(nch)::value, W, decltype(odd)::value>
+    norm_fwd_kernel<TX, TY, N, L, decltype(odd)::value>
         <<<(unsigned)(need < most ? need : most), threads, 0, s>>>(a);
     return hipGetLastError();
   });
@@ -844,13 +911,13 @@ hipError_t norm_bwd_t(
       KFAC_HIP_CHECK(hipGetLastError());
     }
   } else {
-    KFAC_HIP_CHECK(by_width<false>(D, [&](auto nch, auto waves, auto odd) {
-      constexpr int N = decltype(nch)::value, W = decltype(waves)::value;
+    KFAC_HIP_CHECK(by_width<false>(D, [&](auto nch, auto lanes, auto odd) {
+      constexpr int N = decltype(nch)::value, L = decltype(lanes)::value;
       constexpr bool ODD = decltype(odd)::value;
       if (x != nullptr) {
-        norm_bwd_kernel<TX, TY, N, W, ODD, false><<<P, 1024, 0, s>>>(a);
+        norm_bwd_kernel<TX, TY, N, L, ODD, false><<<P, 1024, 0, s>>>(a);
       } else {
-        norm_bwd_kernel<TX, TY, N, W, ODD, true><<<P, 1024, 0, s>>>(a);
+        norm_bwd_kernel<TX, TY, N, L, ODD, true><<<P, 1024, 0, s>>>(a);
       }
       return hipGetLastError();
     }));

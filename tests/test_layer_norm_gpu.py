@@ -100,7 +100,7 @@ def test_types(inner, outer, width) -> None:
 
 
 @pytest.mark.parametrize('rows', [1, 16, 17, 63, 64, 65, 4096, 5000, 20000])
-@pytest.mark.parametrize('width', [24, 600, 1500])
+@pytest.mark.parametrize('width', [24, 64, 100, 250, 256, 600, 1500])
 def test_rows(rows, width) -> None:
     check(rand(rows, width), rand(width), rand(width))
 
