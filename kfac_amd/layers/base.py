@@ -87,6 +87,7 @@ class KFACBaseLayer:
         # flight; held so autograd cannot free them early. Cleared by the
         # preconditioner after joining the side stream.
         self._pending_inputs: list[torch.Tensor] = []
+        self._pending_grads: list[torch.Tensor] = []
 
         # Persistent accumulators for the current batch (fp32).
         self._a_batch: torch.Tensor | None = None
@@ -223,7 +224,7 @@ class KFACBaseLayer:
             s.wait_stream(torch.cuda.current_stream(a.device))
             with torch.cuda.stream(s):
                 self.module.accumulate_a_factor(a, self._a_batch, beta, 1.0)
-            self._hold(a, s)
+            self._hold_input(a, s)
         else:
             self.module.accumulate_a_factor(a, self._a_batch, beta, 1.0)
         self._a_count += 1
@@ -255,13 +256,13 @@ class KFACBaseLayer:
             s.wait_stream(torch.cuda.current_stream(g.device))
             with torch.cuda.stream(s):
                 self.module.accumulate_g_factor(g, self._g_batch, beta, coeff)
-            self._hold(g, s)
+            self._hold_grad(g)
         else:
             self.module.accumulate_g_factor(g, self._g_batch, beta, coeff)
         self._g_count += 1
 
-    def _hold(self, t: torch.Tensor, stream: torch.cuda.Stream) -> None:
-        """Keep ``t``'s memory until the covariance stream has read it.
+    def _hold_input(self, a: torch.Tensor, stream: torch.cuda.Stream) -> None:
+        """Keep ``a``'s memory until the covariance stream has read it.
 
         The reference is dropped in clear_pending() at the step. A module
         that keeps its input in fewer bits (``keeps_codes``) would keep the
@@ -269,9 +270,19 @@ class KFACBaseLayer:
         stream is past the read.
         """
         if getattr(self.module.module, 'keeps_codes', False):
-            t.record_stream(stream)
-            t = t.new_empty(0)
-        self._pending_inputs.append(t)
+            a.record_stream(stream)
+            a = a.new_empty(0)
+        self._pending_inputs.append(a)
+
+    def _hold_grad(self, g: torch.Tensor) -> None:
+        """Keep ``g``'s memory and values until the streams are joined.
+
+        The reference itself is what keeps the values: autograd adds later
+        gradients in place into a tensor that nothing else refers to (a
+        residual branch hands one tensor to its linear and to its sum), on
+        a stream that does not wait for the covariance's read.
+        """
+        self._pending_grads.append(g)
 
     def _factor_ctx(self) -> Any:
         """Stream context for factor EMA/reduce ops.
@@ -282,19 +293,19 @@ class KFACBaseLayer:
         stream (pending list cleared), plain current-stream execution is
         correct.
         """
-        if self._pending_inputs and self._pending_inputs[0].is_cuda:
+        pending = self._pending_inputs or self._pending_grads
+        if pending and pending[0].is_cuda:
             from kfac_amd.streams import cov_stream
 
-            return torch.cuda.stream(
-                cov_stream(self._pending_inputs[0].device),
-            )
+            return torch.cuda.stream(cov_stream(pending[0].device))
         import contextlib
 
         return contextlib.nullcontext()
 
     def clear_pending(self) -> None:
-        """Release input refs after the cov stream has been joined."""
+        """Release the refs after the cov stream has been joined."""
         self._pending_inputs.clear()
+        self._pending_grads.clear()
 
     def reset_batch(self) -> None:
         """Drop accumulated batch contributions (buffers are kept)."""

@@ -198,6 +198,46 @@ def test_kfac_factors_see_the_exact_input() -> None:
         torch.testing.assert_close(a, factors[1][n], rtol=1e-4, atol=1e-5)
 
 
+class Residual(torch.nn.Module):
+    """A block whose output's gradient goes to its linear and past it."""
+
+    def __init__(self) -> None:
+        super().__init__()
+        self.norm = LayerNorm8(64)
+        self.lin = Linear8(64, 64)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        self.stream = x * 1
+        return self.stream + self.lin(self.norm(self.stream).y)
+
+
+def test_output_gradient_stays_until_the_step() -> None:
+    # A covariance may read a linear's output gradient long after the hook:
+    # what the layer holds of it must keep autograd from adding the norm's
+    # gradient into the same tensor, which it does where it has the only
+    # reference.
+    model = Residual()
+    precon = kfac_amd.KFACPreconditioner(model)
+    ((_, layer),) = precon._layers.values()
+    seen = {}
+
+    def accumulate(g, *args) -> None:
+        seen['at'], seen['values'] = g.data_ptr(), g.clone()
+        layer._hold_grad(g)
+
+    layer.module.accumulate_g_factor = accumulate
+    x = torch.randn(5, 64, requires_grad=True)
+    y = model(x)
+    model.stream.register_hook(lambda g: seen.update(total=g.data_ptr()))
+    (y * torch.randn(5, 64)).sum().backward()
+    assert seen['total'] != seen['at']
+    (held,) = layer._pending_grads
+    assert held.data_ptr() == seen['at'] and held._version == 0
+    assert torch.equal(held, seen['values'])
+    layer.clear_pending()
+    assert not layer._pending_grads
+
+
 def test_modules_refuse() -> None:
     with pytest.raises(ValueError):
         LayerNorm8((4, 8))

@@ -112,6 +112,41 @@ def test_kfac_factors_match_the_exact_model() -> None:
         torch.testing.assert_close(a, factors[1][n], rtol=1e-3, atol=1e-4)
 
 
+def test_kfac_output_factors_match_the_exact_model() -> None:
+    # attention's output projection too: its output gradient is the residual
+    # stream's, into which the norm's gradient is added later
+    tokens = torch.randint(0, 997, (16, 128), device='cuda')
+    factors = []
+    for m in models():
+        m.cuda()
+        precon = kfac_amd.KFACPreconditioner(m, skip_layers=['embed_out'])
+        names = {name for name, _ in precon._layers.values()}
+        assert 'layers.0.attention.dense' in names
+        for i in range(3):
+            m(tokens).square().mean().backward()
+            for _, layer in precon._layers.values():
+                assert len(layer._pending_grads) == 1
+                assert layer._pending_grads[0].numel() > 0
+            if i < 2:
+                precon.step()
+                for _, layer in precon._layers.values():
+                    assert not layer._pending_grads
+                m.zero_grad()
+        torch.cuda.synchronize()
+        factors.append(
+            {n: layer.g_factor for n, layer in precon._layers.values()},
+        )
+    # An output gradient g is off by d = 1.2 % from each of the up to 8 kept
+    # tensors behind it, at random: entries of g^T g over M = 2048 tokens by
+    # d * sqrt(2 M) of a product where the diagonal has M of them, and with
+    # N < 800 columns the whole by d * sqrt(2 N / M) < d, and d^2 on the
+    # diagonal. The identity that a factor starts from is left out.
+    for n, g in factors[0].items():
+        eye = 0.95**3 * torch.eye(g.shape[0], device='cuda')
+        off = float((g - factors[1][n]).norm() / (g - eye).norm())
+        assert off < 2 * 0.012 * math.sqrt(8), (n, off)
+
+
 def test_keeps_less_memory() -> None:
     tokens = torch.randint(0, 997, (16, 128), device='cuda')
     kept = []
