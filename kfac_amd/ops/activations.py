@@ -19,6 +19,7 @@ from typing import Any
 from typing import NamedTuple
 
 import torch
+import torch.autograd.forward_ad as fwAD
 import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
@@ -246,11 +247,16 @@ class _GELU8(torch.autograd.Function):
         packed_output: bool,
     ) -> tuple[torch.Tensor, ...]:
         f = gelu8_forward(
-            x, approximate=approximate, packed_output=packed_output,
+            x,
+            approximate=approximate,
+            packed_input=ctx.needs_input_grad[0],
+            packed_output=packed_output,
         )
-        assert f.packed_input is not None
-        ctx.save_for_backward(*f.packed_input)
+        if f.packed_input is not None:
+            ctx.save_for_backward(*f.packed_input)
+        ctx.save_for_forward(x)  # for jvp only, which runs at once
         ctx.approximate = approximate
+        ctx.packed_output = packed_output
         ctx.set_materialize_grads(False)
         if f.packed_output is None:
             return (f.y,)
@@ -267,6 +273,13 @@ class _GELU8(torch.autograd.Function):
         )
         return dx, None, None
 
+    @staticmethod
+    def jvp(ctx: Any, dx: torch.Tensor, *_: Any) -> Any:
+        # the exact input is there: its slope, in elementary operations
+        (x,) = ctx.saved_tensors
+        dy = ref.gelu_backward(dx, x, ctx.approximate)
+        return (dy, None, None) if ctx.packed_output else dy
+
 
 def gelu8(
     x: torch.Tensor,
@@ -277,9 +290,13 @@ def gelu8(
     """GELU that keeps its input in 8 bits for the backward pass.
 
     Returns ``(y, packed)``: ``packed`` is y's 8 bit form for the next
-    :func:`linear8` if ``packed_output`` asks for it, else None.
+    :func:`linear8` if ``packed_output`` asks for it, else None. Forward
+    mode's tangents are those of the exact input.
     """
-    if not (torch.is_grad_enabled() and x.requires_grad):
+    backward = torch.is_grad_enabled() and x.requires_grad
+    # the kernels carry no tangents, the CPU's elementary operations do
+    forward = x.is_cuda and fwAD.unpack_dual(x).tangent is not None
+    if not backward and not forward:
         f = gelu8_forward(
             x,
             approximate=approximate,

@@ -6,6 +6,8 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
+import torch.nn.functional as F
 
 from kfac_amd import ops
 from testing import plain
@@ -123,6 +125,45 @@ def test_gelu8_every_sixteen_bit_value(dtype, approximate) -> None:
     slope = plain.gelu_slope(x8.clamp(-1e6, 1e6), approximate)
     off = 16 * plain.UNIT * (1 + x8.abs().clamp(max=40))
     plain.assert_within(dx, slope, off)
+
+
+@pytest.mark.parametrize('approximate', ['none', 'tanh'])
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('needs_grad', [False, True])
+@pytest.mark.parametrize('packed_output', [False, True])
+def test_gelu8_forward_mode(
+    dtype, approximate, needs_grad, packed_output,
+) -> None:
+    x = (3 * rand(5, 100)).to(dtype)
+    dx = rand(5, 100).to(dtype)
+    want = dx.double() * plain.gelu_slope(x.double(), approximate)
+    off = 16 * plain.UNIT * dx.double().abs() * (1 + x.double().abs())
+    alone, _ = ops.gelu8(x, approximate=approximate)
+    x.requires_grad_(needs_grad)
+    with fwAD.dual_level():
+        y, packed = ops.gelu8(
+            fwAD.make_dual(x, dx),
+            approximate=approximate,
+            packed_output=packed_output,
+        )
+        y, dy = fwAD.unpack_dual(y)
+    assert torch.equal(y, alone)
+    assert y.requires_grad == needs_grad
+    assert (packed is not None) == packed_output
+    plain.assert_within(dy.detach(), want, off)
+
+
+def test_other_forward_mode() -> None:
+    x, dx, w = rand(5, 64), rand(5, 64), rand(3, 64)
+    with fwAD.dual_level():
+        dual = fwAD.make_dual(x, dx)
+        dy = fwAD.unpack_dual(ops.linear8(dual, w)).tangent
+        # no tangent is dropped in silence
+        with pytest.raises(RuntimeError):
+            ops.linear8(dual, w.clone().requires_grad_())
+        with pytest.raises(RuntimeError):
+            ops.layer_norm(dual)
+    assert torch.equal(dy, F.linear(dx, w))
 
 
 @pytest.mark.parametrize('dtype', TYPES)
