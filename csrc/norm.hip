@@ -329,7 +329,7 @@ struct Backward {
                    // or a single block writes it
   void* dw;        // either may be null
   void* db;
-  int type;        // of both
+  int dw_type, db_type;
   long R;
   int D;
   int blocks;
@@ -531,9 +531,9 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(Backward<TX, TY> a) {
     if (!single) {
       a.partial[((long)blockIdx.x * 2 + which) * a.D + col] = v;
     } else if (which && a.db != nullptr) {
-      store_any(a.db, a.type, col, v);
+      store_any(a.db, a.db_type, col, v);
     } else if (!which && a.dw != nullptr) {
-      store_any(a.dw, a.type, col, v);
+      store_any(a.dw, a.dw_type, col, v);
     }
   };
   if (G == 1) {
@@ -585,8 +585,9 @@ __global__ __launch_bounds__(1024) void norm_param_kernel(
     int P,
     int D,
     void* dw,
+    int dw_type,
     void* db,
-    int type) {
+    int db_type) {
   __shared__ float lds[16][kWave];
   const int which = blockIdx.y;
   void* out = which ? db : dw;
@@ -607,7 +608,7 @@ __global__ __launch_bounds__(1024) void norm_param_kernel(
     s = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) s += lds[i][lane];
-    store_any(out, type, c, s);
+    store_any(out, which ? db_type : dw_type, c, s);
   }
 }
 
@@ -893,13 +894,14 @@ hipError_t norm_bwd_t(
     TX* dx,
     float* partial,
     void* dw,
+    int dw_type,
     void* db,
-    int type,
+    int db_type,
     long R,
     int D) {
-  Backward<TX, TY> a{dy, x,       codes, exps, mean, rstd, {w, w_type}, dt,
-                     dx, partial, dw,    db,   type, R,    D,
-                     ceil_div(D, kBlock8)};
+  Backward<TX, TY> a{dy, x,       codes, exps, mean,    rstd,    {w, w_type},
+                     dt, dx,      partial, dw, db,      dw_type, db_type,
+                     R,  D,       ceil_div(D, kBlock8)};
   const int P = norm_bwd_blocks(R, D);
   if (is_long(D)) {
     norm_bwd_long_kernel<TX, TY><<<long_blocks(R), 1024, 0, s>>>(a);
@@ -923,7 +925,7 @@ hipError_t norm_bwd_t(
   }
   if (partial == nullptr) return hipSuccess;
   norm_param_kernel<<<dim3(ceil_div(D, kWave), 2), 1024, 0, s>>>(
-      partial, P, D, dw, db, type);
+      partial, P, D, dw, dw_type, db, db_type);
   return hipGetLastError();
 }
 
@@ -935,7 +937,7 @@ hipError_t norm_bwd_t(
   template hipError_t norm_bwd_t<TX, TY>(                                     \
       hipStream_t, const TY*, const TX*, const int8_t*, const uint8_t*,       \
       const float*, const float*, const void*, int, const TX*, TX*, float*,   \
-      void*, void*, int, long, int);
+      void*, int, void*, int, long, int);
 KFAC_NORM(float, float)
 KFAC_NORM(float, __hip_bfloat16)
 KFAC_NORM(float, __half)

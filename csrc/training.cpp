@@ -344,7 +344,8 @@ std::tuple<Tensor, OptTensor, OptTensor> norm_backward(
     const OptTensor& w,
     bool want_db,
     const OptTensor& dt,
-    std::optional<torch::ScalarType> dtype) {
+    std::optional<torch::ScalarType> dtype,
+    std::optional<torch::ScalarType> bias_dtype) {
   const Shape s = check_rows(dy, "dy");
   auto xt = dy.scalar_type();
   if (total) {
@@ -373,20 +374,22 @@ std::tuple<Tensor, OptTensor, OptTensor> norm_backward(
     TORCH_CHECK_TYPE(
         dt->scalar_type() == xt, "grad_total must be ", xt, ", as dx is");
   }
+  check_float(bias_dtype.value_or(torch::kFloat32), "bias_dtype");
   const c10::DeviceGuard guard(dy.device());
   const Borrowed dc = dy.expect_contiguous();
   const Borrowed mc = mean.expect_contiguous(), rc = rstd.expect_contiguous();
   const Param xp(total), cp(codes), ep(exps), wp(w), tp(dt);
   auto dx = empty(dy.sizes(), xt, dy);
-  const auto pt = w ? w->scalar_type() : torch::kFloat32;
+  const auto wt = w ? w->scalar_type() : torch::kFloat32;
+  const auto bt = bias_dtype.value_or(wt);
   OptTensor dw, db;
   if (s.R == 0) {
-    if (w) dw = zeros({s.D}, pt, dy);
-    if (want_db) db = zeros({s.D}, pt, dy);
+    if (w) dw = zeros({s.D}, wt, dy);
+    if (want_db) db = zeros({s.D}, bt, dy);
     return {dx, dw, db};
   }
-  if (w) dw = empty({s.D}, pt, dy);
-  if (want_db) db = empty({s.D}, pt, dy);
+  if (w) dw = empty({s.D}, wt, dy);
+  if (want_db) db = empty({s.D}, bt, dy);
   Tensor partial;
   const long rows = dw || db ? kfac::norm_bwd_partials(s.R, s.D) : 0;
   if (rows > 0) partial = empty({rows * 2 * s.D}, torch::kFloat32, dy);
@@ -400,8 +403,8 @@ std::tuple<Tensor, OptTensor, OptTensor> norm_backward(
         (const float*)rc->const_data_ptr(), wp.p, wp.type, (const TX*)tp.p,
         (TX*)dx.data_ptr(),
         partial.defined() ? (float*)partial.data_ptr() : nullptr,
-        dw ? dw->data_ptr() : nullptr, db ? db->data_ptr() : nullptr,
-        type_of(pt), s.R, s.D)));
+        dw ? dw->data_ptr() : nullptr, type_of(wt),
+        db ? db->data_ptr() : nullptr, type_of(bt), s.R, s.D)));
   });
   return {std::move(dx), std::move(dw), std::move(db)};
 }
@@ -412,7 +415,8 @@ std::tuple<Tensor, OptTensor> weight_grad8(
     const Tensor& codes,
     const Tensor& exps,
     bool want_bias,
-    torch::ScalarType dtype) {
+    torch::ScalarType dtype,
+    std::optional<torch::ScalarType> bias_dtype) {
   const Shape sg = check_rows(g, "g");
   const Shape sx = check_packed(codes, exps);
   TORCH_CHECK_VALUE(
@@ -423,6 +427,8 @@ std::tuple<Tensor, OptTensor> weight_grad8(
       g.sizes(), " on ", g.device(), " and ", codes.sizes(), " on ",
       codes.device());
   check_float(dtype, "dtype");
+  const auto bt = bias_dtype.value_or(dtype);
+  check_float(bt, "bias_dtype");
   const c10::DeviceGuard guard(g.device());
   const Borrowed gc = g.expect_contiguous();
   const Borrowed cc = codes.expect_contiguous(), ec = exps.expect_contiguous();
@@ -433,11 +439,11 @@ std::tuple<Tensor, OptTensor> weight_grad8(
       "a weight gradient takes rows of less than 2^27 values");
   OptTensor db;
   if (M == 0) {
-    if (want_bias) db = zeros({N}, dtype, g);
+    if (want_bias) db = zeros({N}, bt, g);
     return {zeros({N, K}, dtype, g), db};
   }
   auto dw = empty({N, K}, dtype, g);
-  if (want_bias) db = empty({N}, dtype, g);
+  if (want_bias) db = empty({N}, bt, g);
   const auto stream = stream_of(g);
   by_type(g.scalar_type(), [&](auto t) {
     using T = decltype(t);
@@ -445,7 +451,7 @@ std::tuple<Tensor, OptTensor> weight_grad8(
     const long rows = (long)plan.splits * plan.bias_tiles;
     // a single fp32 sum is the result itself; the others share a workspace
     const bool direct = plan.splits == 1 && dtype == torch::kFloat32;
-    const bool bias_direct = rows == 1 && dtype == torch::kFloat32;
+    const bool bias_direct = rows == 1 && bt == torch::kFloat32;
     const long need = direct ? 0 : plan.splits * N * K;
     const long bias_need = want_bias && !bias_direct ? rows * N : 0;
     Tensor work;
@@ -463,8 +469,8 @@ std::tuple<Tensor, OptTensor> weight_grad8(
         bias));
     CHECK_OK(kfac::wgrad8_add(
         stream, sums, plan.splits, N * K, need ? dw.data_ptr() : nullptr,
-        bias, (int)rows, N, bias_need ? db->data_ptr() : nullptr,
-        type_of(dtype)));
+        type_of(dtype), bias, (int)rows, N,
+        bias_need ? db->data_ptr() : nullptr, type_of(bt)));
   });
   return {std::move(dw), std::move(db)};
 }

@@ -50,8 +50,8 @@ template <typename TX, typename TY>
 hipError_t norm_bwd_t(
     hipStream_t, const TY* dy, const TX* x, const int8_t* codes,
     const uint8_t* exps, const float* mean, const float* rstd, const void* w,
-    int w_type, const TX* dt, TX* dx, float* partial, void* dw, void* db,
-    int type, long R, int D);
+    int w_type, const TX* dt, TX* dx, float* partial, void* dw, int dw_type,
+    void* db, int db_type, long R, int D);
 
 // How a weight gradient is cut into blocks.
 struct WGradPlan {
@@ -72,7 +72,7 @@ hipError_t wgrad8_t(
 // bias; either output may be null
 hipError_t wgrad8_add(
     hipStream_t, const float* sums, int splits, long n, void* out,
-    const float* bias_sums, int bias_rows, long bias_n, void* bias_out,
-    int type);
+    int type, const float* bias_sums, int bias_rows, long bias_n,
+    void* bias_out, int bias_type);
 
 }  // namespace kfac

@@ -646,12 +646,14 @@ hipError_t wgrad8_add(
     int splits,
     long n,
     void* out,
+    int type,
     const float* bias_sums,
     int bias_rows,
     long bias_n,
     void* bias_out,
-    int type) {
-  const auto sum_of = [&](const float* parts, void* o, long n, int rows) {
+    int bias_type) {
+  const auto sum_of = [](
+      const float* parts, void* o, long n, int rows, int type) {
     Sum a{parts, o, o == nullptr ? 0 : n, rows, type, 1, 0};
     // kTurn rows a thread at most, and two blocks for each compute unit as long
     // as a thread has 2 rows or more
@@ -665,8 +667,9 @@ hipError_t wgrad8_add(
     a.blocks = (unsigned)(need < (1 << 20) ? need : 1 << 20);
     return a;
   };
-  const Sum weight = sum_of(sums, out, n, splits);
-  const Sum bias = sum_of(bias_sums, bias_out, bias_n, bias_rows);
+  const Sum weight = sum_of(sums, out, n, splits, type);
+  const Sum bias =
+      sum_of(bias_sums, bias_out, bias_n, bias_rows, bias_type);
   if (weight.blocks + bias.blocks == 0) return hipSuccess;
   wgrad8_add_kernel<<<weight.blocks + bias.blocks, 256, 0, s>>>(weight, bias);
   return hipGetLastError();

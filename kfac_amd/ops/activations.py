@@ -207,6 +207,7 @@ def weight_grad8(
     *,
     bias: bool = True,
     dtype: torch.dtype = torch.float32,
+    bias_dtype: torch.dtype | None = None,
 ) -> tuple[torch.Tensor, torch.Tensor | None]:
     """A linear layer's weight and bias gradient from its 8 bit input.
 
@@ -214,14 +215,15 @@ def weight_grad8(
     of the layer's output, (..., N); ``packed_input`` holds the layer's
     input, (..., K), with as many rows. Every product is exact and sums are
     kept in float32 for each type of ``g``; the results, (N, K) and (N,),
-    are rounded once to ``dtype``. Without rows they are zero. The same
-    inputs give the same bits each time. N and K are below 2^27.
+    are rounded once, to ``dtype`` and ``bias_dtype`` (by default the same).
+    Without rows they are zero. The same inputs give the same bits each time.
+    N and K are below 2^27.
     """
     codes, exps = packed_input
     if g.is_cuda:
         ext = ops._require_ext('weight_grad8')
         if ext is not None:
-            return ext.weight_grad8(g, codes, exps, bias, dtype)
+            return ext.weight_grad8(g, codes, exps, bias, dtype, bias_dtype)
     check_rows(g, 'g')
     check_packed(packed_input)
     if g.shape[:-1] != codes.shape[:-1] or g.device != codes.device:
@@ -230,9 +232,13 @@ def weight_grad8(
             f'{tuple(g.shape)} on {g.device} and {tuple(codes.shape)} on '
             f'{codes.device}',
         )
-    if dtype not in FLOAT_TYPES:
-        raise TypeError(f'no gradients of type {dtype}')
-    return ref.weight_grad(g, ref.unpack8(codes, exps), bias, dtype)
+    bias_dtype = dtype if bias_dtype is None else bias_dtype
+    for t in (dtype, bias_dtype):
+        if t not in FLOAT_TYPES:
+            raise TypeError(f'no gradients of type {t}')
+    return ref.weight_grad(
+        g, ref.unpack8(codes, exps), bias, dtype, bias_dtype,
+    )
 
 
 # -- autograd ----------------------------------------------------------------
@@ -341,11 +347,14 @@ class _Linear8(torch.autograd.Function):
             if ctx.needs_input_grad[0]:
                 dx = g @ weight.to(ctx.dtype)
         if ctx.needs_input_grad[1]:
+            # a bias of another type (float64, say) takes the float32 sum
+            own = ctx.bias_dtype in FLOAT_TYPES
             dw, db = weight_grad8(
                 g,
                 Packed8(*packed),
                 bias=ctx.needs_input_grad[2],
                 dtype=weight.dtype,
+                bias_dtype=ctx.bias_dtype if own else torch.float32,
             )
         elif ctx.needs_input_grad[2]:
             db = g.reshape(-1, g.shape[-1]).sum(0, dtype=torch.float32)

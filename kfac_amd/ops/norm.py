@@ -148,6 +148,7 @@ def layer_norm_backward(
     bias: bool = True,
     grad_total: torch.Tensor | None = None,
     dtype: torch.dtype | None = None,
+    bias_dtype: torch.dtype | None = None,
 ) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor | None]:
     """Gradients of :func:`layer_norm_forward`: (dx, dweight, dbias).
 
@@ -160,10 +161,11 @@ def layer_norm_backward(
         bias: whether to return the bias's gradient.
         grad_total: gradient that reaches the sum past the norm; added.
         dtype: dx's type, total's if that is a tensor, else by default dy's.
+        bias_dtype: dbias's type, by default dweight's.
 
     dx is the gradient of the sum, hence of x and of the residual alike.
-    The parameters' gradients come in the weight's type (float32 without a
-    weight). The same inputs give the same bits each time.
+    dweight comes in the weight's type (float32 without a weight). The same
+    inputs give the same bits each time.
     """
     packed = not isinstance(total, torch.Tensor)
     if dy.is_cuda:
@@ -180,6 +182,7 @@ def layer_norm_backward(
                 bias,
                 grad_total,
                 dtype,
+                bias_dtype,
             )
     check_rows(dy, 'dy')
     if packed:
@@ -206,16 +209,19 @@ def layer_norm_backward(
         check_same_shape(dy, grad_total, 'dy and grad_total')
         if grad_total.dtype != dtype:
             raise TypeError(f'grad_total must be {dtype}, as dx is')
+    wtype = torch.float32 if weight is None else weight.dtype
+    bias_dtype = wtype if bias_dtype is None else bias_dtype
+    if bias_dtype not in FLOAT_TYPES:
+        raise TypeError(f'no gradients of type {bias_dtype}')
     if packed:
         total = ref.unpack8(*total)
     dx, dw, db = ref.layer_norm_backward(
         dy, total, mean, rstd, weight, grad_total, dtype,
     )
-    ptype = torch.float32 if weight is None else weight.dtype
     return (
         dx,
-        None if weight is None else dw.to(ptype),
-        db.to(ptype) if bias else None,
+        None if weight is None else dw.to(wtype),
+        db.to(bias_dtype) if bias else None,
     )
 
 
@@ -273,9 +279,8 @@ class _LayerNorm(torch.autograd.Function):
                 bias=want[3],
                 grad_total=dt,
                 dtype=ctx.dtype,
+                bias_dtype=ctx.bias_dtype,
             )
-            if db is not None:
-                db = db.to(ctx.bias_dtype)
         dr = None
         if ctx.residual_dtype is not None and dx is not None:
             dr = dx.to(ctx.residual_dtype)

@@ -281,11 +281,12 @@ def weight_grad(
     a: torch.Tensor,
     bias: bool,
     dtype: torch.dtype,
+    bias_dtype: torch.dtype,
 ) -> tuple[torch.Tensor, torch.Tensor | None]:
     """(g^T a, column sums of g) over all rows, summed in fp32."""
     g32 = g.to(torch.float32).reshape(-1, g.shape[-1])
     a32 = a.to(torch.float32).reshape(-1, a.shape[-1])
-    db = g32.sum(0).to(dtype) if bias else None
+    db = g32.sum(0).to(bias_dtype) if bias else None
     return (g32.t() @ a32).to(dtype), db
 
 

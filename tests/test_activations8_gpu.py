@@ -247,6 +247,37 @@ def test_no_rows() -> None:
     assert torch.equal(db, torch.zeros(5, device='cuda', dtype=BF16))
 
 
+@pytest.mark.parametrize('m,n,k', [(1, 3, 5), (4096, 33, 70), (16384, 63, 519), (300, 768, 768)])
+def test_parameters_of_two_types(m, n, k) -> None:
+    # each gradient is the float32 sum, rounded once to its own type
+    f32, bf16, f16 = TYPES
+    x, g = rand(m, k), 1 + rand(m, n)
+    for xt, bt in ((bf16, f32), (f32, bf16), (f16, bf16)):
+        p = ops.pack8(x.to(xt))
+        want = plain.weight_grads(g.to(xt), ops.unpack8(p).double())
+        w = rand(n, k).to(xt).requires_grad_()
+        b = rand(n).to(bt).requires_grad_()
+        ops.linear8(x.to(xt), w, b).backward(g.to(xt))
+        assert (w.grad.dtype, b.grad.dtype) == (xt, bt)
+        plain.assert_within(w.grad, *want['dw'])
+        plain.assert_within(b.grad, *want['db'])
+        dw, db = ops.weight_grad8(g.to(xt), p, dtype=xt, bias_dtype=bt)
+        assert torch.equal(dw, w.grad) and torch.equal(db, b.grad)
+    # of a type that the operators do not have: from the float32 sum
+    b = rand(n).double().requires_grad_()
+    ops.linear8(x, w.detach().float().requires_grad_(), b).backward(g)
+    assert b.grad.dtype == torch.float64
+    want = plain.weight_grads(g, ops.unpack8(p).double())
+    plain.assert_within(b.grad.float(), *want['db'])
+    with pytest.raises(TypeError):
+        ops.weight_grad8(g, p, bias_dtype=torch.float64)
+    dw, db = ops.weight_grad8(
+        g[:0], ops.pack8(x[:0]), dtype=f16, bias_dtype=f32,
+    )
+    assert (dw.dtype, db.dtype) == (f16, f32)
+    assert not dw.any() and not db.any()
+
+
 def test_linear8_training_step() -> None:
     x = rand(64, 20, 256).requires_grad_()
     w = (rand(512, 256) / 16).requires_grad_()

@@ -147,6 +147,40 @@ def test_no_rows_and_constant_rows() -> None:
     assert torch.equal(n.y, b.expand(2, 5))
 
 
+@pytest.mark.parametrize('rows', [1, 4096])
+@pytest.mark.parametrize('width', [70])
+def test_parameters_of_two_types(rows, width) -> None:
+    # each gradient is the float32 sum, rounded once to its own type
+    x, dy = torch.randn(rows, width), 1 + torch.randn(rows, width)
+    for wt, bt in ((BF16, F32), (F32, BF16), (F16, BF16)):
+        w, b = torch.randn(width).to(wt), torch.randn(width).to(bt)
+        n = ops.layer_norm_forward(x, w, b)
+        want = plain.norm_grads(dy, x, n.mean, n.rstd, w, None)
+        w.requires_grad_(), b.requires_grad_()
+        ops.layer_norm(x, w, b).y.backward(dy)
+        assert (w.grad.dtype, b.grad.dtype) == (wt, bt)
+        plain.assert_within(w.grad, *want['dw'])
+        plain.assert_within(b.grad, *want['db'])
+        _, dw, db = ops.layer_norm_backward(
+            dy, x, n.mean, n.rstd, w.detach(), bias_dtype=bt,
+        )
+        assert torch.equal(dw, w.grad) and torch.equal(db, b.grad)
+    _, dw, db = ops.layer_norm_backward(
+        dy, x, n.mean, n.rstd, bias_dtype=BF16,
+    )
+    assert dw is None and db.dtype == BF16
+    plain.assert_within(db, *want['db'])
+    with pytest.raises(TypeError):
+        ops.layer_norm_backward(
+            dy, x, n.mean, n.rstd, bias_dtype=torch.float64,
+        )
+    none = ops.layer_norm_backward(
+        dy[:0], x[:0], n.mean[:0], n.rstd[:0], w.detach(), bias_dtype=F32,
+    )
+    assert none[1].dtype == F16 and none[2].dtype == F32
+    assert not none[1].any() and not none[2].any()
+
+
 def test_refusals() -> None:
     x = torch.randn(4, 10)
     w = torch.randn(10)
