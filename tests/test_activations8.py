@@ -271,6 +271,41 @@ def test_linear8_autocast() -> None:
     plain.assert_within(w.grad, *exact['dw'])
 
 
+def test_autocast_around_everything() -> None:
+    # autocast chooses linear8's type and nothing else
+    x, g = torch.randn(50, 70), torch.randn(50, 33)
+    w = torch.randn(33, 70, requires_grad=True)
+    b = torch.randn(33, requires_grad=True)
+    norm = torch.randn(70), torch.randn(70)
+
+    def passes() -> list[torch.Tensor]:
+        p = ops.pack8(x)
+        out = [*p, ops.unpack8(p), *ops.weight_grad8(g, p)]
+        for form in ('none', 'tanh'):
+            f = ops.gelu8_forward(x, approximate=form)
+            out += [f.y, ops.gelu8_backward(x, p, approximate=form)]
+        n = ops.layer_norm_forward(x, *norm)
+        out += [n.y, n.mean, n.rstd]
+        return out + [
+            *ops.layer_norm_backward(x, p, n.mean, n.rstd, norm[0]),
+        ]
+
+    def gradients(inside: bool) -> tuple[torch.Tensor, ...]:
+        with torch.autocast('cpu', dtype=torch.bfloat16):
+            y = ops.linear8(x, w, b)
+            if inside:
+                return torch.autograd.grad(y, (w, b), g.to(y.dtype))
+        return torch.autograd.grad(y, (w, b), g.to(y.dtype))
+
+    want = passes()
+    with torch.autocast('cpu', dtype=torch.bfloat16):
+        got = passes()
+    for i, (p, q) in enumerate(zip(got, want)):
+        assert torch.equal(p, q), i
+    for p, q in zip(gradients(True), gradients(False)):
+        assert torch.equal(p, q)
+
+
 def test_linear8_takes_packed_input() -> None:
     x = torch.randn(4, 70)
     w = torch.randn(3, 70, requires_grad=True)

@@ -295,6 +295,16 @@ def test_linear8_training_step() -> None:
     plain.assert_within(db, *exact['db'])
 
 
+def test_linear8_backward_under_autocast() -> None:
+    x, g = rand(200, 256), rand(200, 300).bfloat16()
+    w, b = rand(300, 256).requires_grad_(), rand(300).requires_grad_()
+    with torch.autocast('cuda', dtype=BF16):
+        y = ops.linear8(x, w, b)
+        inside = torch.autograd.grad(y, (w, b), g, retain_graph=True)
+    for p, q in zip(inside, torch.autograd.grad(y, (w, b), g)):
+        assert torch.equal(p, q)
+
+
 def test_expanded_gradient() -> None:
     x = rand(30, 100).requires_grad_()
     w, b = rand(70, 100).requires_grad_(), rand(70).requires_grad_()
