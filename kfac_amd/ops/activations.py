@@ -374,7 +374,8 @@ def linear8(
 
     The result is that of ``torch.nn.functional.linear`` (under autocast in
     autocast's type); the weight's gradient comes from the codes.
-    ``packed`` is the 8 bit form of ``x`` if the op before has made it
+    The bias may be of another type than ``x`` and ``weight``. ``packed`` is
+    the 8 bit form of ``x`` if the op before has made it
     (``packed_output``), which saves the pass that packs it here. Without a
     gradient to compute nothing is packed.
     """
@@ -400,6 +401,7 @@ def linear8(
         weight.requires_grad or x.requires_grad
         or (bias is not None and bias.requires_grad)
     ):
-        return F.linear(x, weight, bias)
+        # torch casts the bias itself under autocast only
+        return F.linear(x, weight, None if bias is None else bias.to(dtype))
     codes, exps = packed if packed is not None else (None, None)
     return _Linear8.apply(x, weight, bias, codes, exps, dtype)

@@ -278,6 +278,23 @@ def test_parameters_of_two_types(m, n, k) -> None:
     assert not dw.any() and not db.any()
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('bias', [*TYPES, torch.float64])
+def test_linear8_bias_type_without_gradients(dtype, bias) -> None:
+    x, w = rand(4, 8).to(dtype), rand(3, 8).to(dtype).requires_grad_()
+    b = rand(3).to(bias).requires_grad_()
+    y = ops.linear8(x, w, b)
+    with torch.no_grad():
+        assert torch.equal(ops.linear8(x, w, b), y)
+    assert torch.equal(ops.linear8(x, w.detach(), b.detach()), y)
+    kind = x.device.type
+    with torch.autocast(kind, dtype=torch.bfloat16):
+        y = ops.linear8(x, w, b)
+        with torch.no_grad():
+            assert torch.equal(ops.linear8(x, w, b), y)
+    assert y.dtype == torch.bfloat16
+
+
 def test_linear8_training_step() -> None:
     x = rand(64, 20, 256).requires_grad_()
     w = (rand(512, 256) / 16).requires_grad_()
