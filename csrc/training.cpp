@@ -342,6 +342,7 @@ std::tuple<Tensor, OptTensor, OptTensor> norm_backward(
     const Tensor& mean,
     const Tensor& rstd,
     const OptTensor& w,
+    bool want_dw,
     bool want_db,
     const OptTensor& dt,
     std::optional<torch::ScalarType> dtype,
@@ -383,12 +384,13 @@ std::tuple<Tensor, OptTensor, OptTensor> norm_backward(
   const auto wt = w ? w->scalar_type() : torch::kFloat32;
   const auto bt = bias_dtype.value_or(wt);
   OptTensor dw, db;
+  want_dw = want_dw && w;
   if (s.R == 0) {
-    if (w) dw = zeros({s.D}, wt, dy);
+    if (want_dw) dw = zeros({s.D}, wt, dy);
     if (want_db) db = zeros({s.D}, bt, dy);
     return {dx, dw, db};
   }
-  if (w) dw = empty({s.D}, wt, dy);
+  if (want_dw) dw = empty({s.D}, wt, dy);
   if (want_db) db = empty({s.D}, bt, dy);
   Tensor partial;
   const long rows = dw || db ? kfac::norm_bwd_partials(s.R, s.D) : 0;

@@ -145,6 +145,7 @@ def layer_norm_backward(
     rstd: torch.Tensor,
     weight: torch.Tensor | None = None,
     *,
+    weight_grad: bool = True,
     bias: bool = True,
     grad_total: torch.Tensor | None = None,
     dtype: torch.dtype | None = None,
@@ -158,6 +159,7 @@ def layer_norm_backward(
         mean: of the forward pass.
         rstd: of the forward pass.
         weight: of the forward pass; without one dweight is None.
+        weight_grad: whether to return the weight's gradient.
         bias: whether to return the bias's gradient.
         grad_total: gradient that reaches the sum past the norm; added.
         dtype: dx's type, total's if that is a tensor, else by default dy's.
@@ -179,6 +181,7 @@ def layer_norm_backward(
                 mean,
                 rstd,
                 weight,
+                weight_grad,
                 bias,
                 grad_total,
                 dtype,
@@ -220,7 +223,7 @@ def layer_norm_backward(
     )
     return (
         dx,
-        None if weight is None else dw.to(wtype),
+        dw.to(wtype) if weight is not None and weight_grad else None,
         db.to(bias_dtype) if bias else None,
     )
 
@@ -276,6 +279,7 @@ class _LayerNorm(torch.autograd.Function):
                 mean,
                 rstd,
                 weight,
+                weight_grad=want[2],
                 bias=want[3],
                 grad_total=dt,
                 dtype=ctx.dtype,

@@ -325,6 +325,39 @@ def test_parameters_of_two_types(rows, width) -> None:
     assert not none[1].any() and not none[2].any()
 
 
+@pytest.mark.parametrize('width', [5, 70, 768, 3000, 17000])
+@pytest.mark.parametrize('rows', [0, 3, 700])
+def test_frozen_parameters(rows, width, monkeypatch) -> None:
+    from kfac_amd.ops import norm
+
+    made = []
+    backward = norm.layer_norm_backward
+
+    def spy(*args, **kwargs):
+        made.append(backward(*args, **kwargs))
+        return made[-1]
+
+    monkeypatch.setattr(norm, 'layer_norm_backward', spy)
+    x, dy = rand(rows, width), rand(rows, width)
+    w, b = rand(width), rand(width)
+    grads = []
+    for frozen in ((), (w,), (b,), (w, b)):
+        x.requires_grad_()
+        for t in (w, b):
+            t.requires_grad_(all(t is not f for f in frozen))
+            t.grad = x.grad = None
+        ops.layer_norm(x, w, b).y.backward(dy)
+        grads.append((x.grad, w.grad, b.grad))
+    for (dx, dw, db), got, skip in zip(
+        grads, made, ((), (1,), (2,), (1, 2)),
+    ):
+        for i, (p, q) in enumerate(zip((dx, dw, db), got)):
+            if i in skip:
+                assert p is None and q is None
+            else:
+                assert torch.equal(p, grads[0][i]) and torch.equal(q, p)
+
+
 def test_refusals() -> None:
     x, w = rand(4, 10), rand(10)
     n = ops.layer_norm_forward(x, w)
