@@ -156,8 +156,11 @@ class GPTNeoXModel(nn.Module):
         self.layers = nn.ModuleList(
             block(d, n_heads, ffn) for _ in range(n_layers)
         )
-        norm = nn.LayerNorm if activation_bits is None else LayerNorm8
-        self.final_layer_norm = norm(d)
+        if activation_bits is None:
+            self.final_layer_norm = nn.LayerNorm(d)
+        else:
+            # embed_out keeps its input as it is
+            self.final_layer_norm = LayerNorm8(d, packed_output=False)
         self.embed_out = nn.Linear(d, vocab, bias=False)
         # weight tying -> 125.3M parameters total at the default config
         self.embed_out.weight = self.embed_in.weight

@@ -21,6 +21,8 @@ class LayerNorm8(nn.LayerNorm):
 
     Keeps the sum in 8 bits for the backward pass. Under autocast the result
     has autocast's type, which the next linear layer computes in.
+    ``packed_output=False`` leaves out the result's 8 bit form, for a norm
+    that no :class:`Linear8` follows.
     """
 
     def __init__(
@@ -29,10 +31,12 @@ class LayerNorm8(nn.LayerNorm):
         eps: float = 1e-5,
         elementwise_affine: bool = True,
         bias: bool = True,
+        packed_output: bool = True,
     ):
         super().__init__(normalized_shape, eps, elementwise_affine, bias)
         if len(self.normalized_shape) != 1:
             raise ValueError('LayerNorm8 takes the last dimension only')
+        self.packed_output = packed_output
 
     def forward(  # type: ignore[override]
         self,
@@ -56,7 +60,7 @@ class LayerNorm8(nn.LayerNorm):
             residual=residual,
             out_dtype=out_dtype,
             keep8=True,
-            packed_output=torch.is_grad_enabled(),
+            packed_output=self.packed_output and torch.is_grad_enabled(),
         )
 
 

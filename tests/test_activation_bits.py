@@ -238,6 +238,24 @@ def test_output_gradient_stays_until_the_step() -> None:
     assert not layer._pending_grads
 
 
+def test_packs_what_is_read(monkeypatch) -> None:
+    from kfac_amd.ops import norm
+
+    asked = []
+    forward = norm.layer_norm_forward
+
+    def spy(*args, **kwargs):
+        asked.append((kwargs['packed_input'], kwargs['packed_output']))
+        return forward(*args, **kwargs)
+
+    monkeypatch.setattr(norm, 'layer_norm_forward', spy)
+    _, model = models()
+    tokens = torch.randint(0, 97, (2, 5))
+    model(tokens)
+    # two norms a block, whose results linears keep, and the last one
+    assert asked == [(True, True)] * 4 + [(True, False)]
+
+
 def test_modules_refuse() -> None:
     with pytest.raises(ValueError):
         LayerNorm8((4, 8))
