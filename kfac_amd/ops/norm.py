@@ -317,7 +317,9 @@ def layer_norm(
     the result continues the residual stream: its gradient joins the norm's
     in one pass.
     """
-    keep8 = keep8 and torch.is_grad_enabled()
+    keep8 = keep8 and torch.is_grad_enabled() and any(
+        t is not None and t.requires_grad for t in (x, residual, weight, bias)
+    )
     y, *more = _LayerNorm.apply(
         x, residual, weight, bias, eps, out_dtype, keep8, packed_output,
     )

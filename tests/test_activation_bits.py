@@ -256,6 +256,34 @@ def test_packs_what_is_read(monkeypatch) -> None:
     assert asked == [(True, True)] * 4 + [(True, False)]
 
 
+def test_keeps_nothing_without_a_gradient(monkeypatch) -> None:
+    from kfac_amd.ops import norm
+
+    asked = []
+    forward = norm.layer_norm_forward
+
+    def spy(*args, **kwargs):
+        asked.append((kwargs['packed_input'], kwargs['packed_output']))
+        return forward(*args, **kwargs)
+
+    monkeypatch.setattr(norm, 'layer_norm_forward', spy)
+    _, model = models()
+    tokens = torch.randint(0, 97, (2, 5))
+    model.requires_grad_(False)
+    model(tokens)
+    with torch.no_grad():
+        model.requires_grad_(True)(tokens)
+    assert not any(packed_input for packed_input, _ in asked)
+    x = torch.randn(3, 8)
+    for i in range(4):
+        args = [x, torch.randn(8), torch.randn(8), x.clone()]
+        args[i].requires_grad_()
+        asked.clear()
+        norm.layer_norm(*args[:3], residual=args[3], keep8=True)
+        assert asked == [(True, False)]
+        x = x.detach()
+
+
 def test_modules_refuse() -> None:
     with pytest.raises(ValueError):
         LayerNorm8((4, 8))
