@@ -127,6 +127,30 @@ def test_gelu8_every_sixteen_bit_value(dtype, approximate) -> None:
     plain.assert_within(dx, slope, off)
 
 
+def test_gelu8_tail() -> None:
+    # Relative errors, in units of 2^-24, where the values themselves are
+    # small. The exponential's argument -x^2 / 2 is rounded three times (a
+    # square and two factors): 1.5 x^2 units, and the instruction is off by 2.
+    # The polynomial is off by 1.4e-7 (3 units), its 7 fmas by at most 2.2
+    # units each (sum of |terms| over their sum), and its argument t by 4,
+    # which t m'(t) / m(t) < 2.5 makes 10: 28. One more for the product.
+    x = torch.linspace(-10, -1, 9001, device='cuda').view(-1, 1)
+    y = ops.gelu8_forward(x).y
+    want = plain.gelu(x.double(), 'none')
+    off = plain.UNIT * (31 + 1.5 * x.double().square()) * want.abs()
+    plain.assert_within(y, want, off)
+    # The slope q - |x| e / sqrt(2 pi), q the tail, from -2 down: the
+    # exponential's errors are common to both terms, 31 units of each others'
+    # (3 roundings of the second) grow by (x^2 + 1) / (x^2 - 1) <= 5 / 3.
+    x = -torch.arange(16, 81, device='cuda').view(-1, 1) / 8  # 7 bits each
+    f = ops.gelu8_forward(x)
+    assert torch.equal(ops.unpack8(f.packed_input), x)
+    dx = ops.gelu8_backward(torch.ones_like(x), f.packed_input)
+    want = plain.gelu_slope(x.double(), 'none')
+    off = plain.UNIT * (54 + 1.5 * x.double().square()) * want.abs()
+    plain.assert_within(dx, want, off)
+
+
 @pytest.mark.parametrize('approximate', ['none', 'tanh'])
 @pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('needs_grad', [False, True])
