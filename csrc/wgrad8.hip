@@ -19,11 +19,12 @@
 // fill the card; the splits' fp32 sums are added by a second kernel in a
 // fixed order.
 //
-// Measured: 16384 tokens x 8192 x 4096 bf16 894 us (1230 TFLOP/s; a product
-// of 8192^3 by the library 1228), bound by the clock that the power limit
-// leaves; 16384 x 768 x 2304 73 us: 50 in the products, 13 to start, end and
-// write 9 splits' sums, and 12 to add these; 8192 x 4096 x 4096 fp32 700 us
-// (393 TFLOP/s, three times that on the matrix cores).
+// Measured, whole calls in a row: 16384 tokens x 8192 x 4096 bf16 900 to 930
+// us by card (1180 to 1220 TFLOP/s; a product of 8192^3 by the library 1228),
+// bound by the clock that the power limit leaves; 16384 x 768 x 2304 74 to 76
+// us: 50 in the products, 13 to start, end and write 9 splits' sums, and 12 to
+// add these; the same in fp16 159 us, in fp32 197; 8192 x 4096 x 4096 fp32 750
+// us (370 TFLOP/s, three times that on the matrix cores).
 
 #include "act8.h"
 
@@ -517,7 +518,7 @@ template <typename TG>
 constexpr int kParts =
     sizeof(TG) == 4 ? 3 : std::is_same<TG, __half>::value ? 2 : 1;
 
-// The tiles of a product: small, large, and for up to 32 outputs narrow ones.
+// The tiles of a product: small, large, and for up to 64 outputs narrow ones.
 // Two images are 128 KB of LDS for large bf16 tiles, one block to a compute
 // unit, and 80 KB or less for the others, two blocks or three.
 enum Tiles { kSmall, kLarge, kNarrow };
