@@ -19,10 +19,11 @@
 // from run to run. Rows longer than 16384 (or shorter than 8) take the kernels
 // at the end of the file, which read a row once for each of its sums.
 //
-// Measured: forward 16384 x 8192 bf16 99 us (5.4 TB/s), 16384 x 768 fp32 and
-// a bf16 residual to bf16 and two 8 bit forms 35 us (5.0 TB/s); backward 146
-// to 159 us (5.1 to 5.5 TB/s) and, from 8 bits, 28 us (4.9 TB/s), with 5 us
-// for the parameters' sums. A copy of 1 GiB reaches 5.2 TB/s.
+// Measured, whole calls in a row: forward 16384 x 8192 bf16 102 us (5.2 TB/s),
+// 16384 x 768 fp32 and a bf16 residual to bf16 and two 8 bit forms 34 us (5.2
+// TB/s); backward 150 us (5.4 TB/s) and, from 8 bits, 29 us (4.7 TB/s), with
+// some 5 us of each for the parameters' sums. A copy of 1 GiB reaches 5.2
+// TB/s.
 
 #include "act8.h"
 
@@ -795,8 +796,13 @@ int rows_of_block(int D) {
 // on that. With HALVED the rows of odd lengths take half the waves and two
 // chunks a lane where they would take 4 to 16 waves: they start at any
 // alignment, such loads take longer, and more of these rows are under way at
-// a time (forward, 6898 x 6697 bf16: 51 us, 72 with 16 waves; 6696: 42 us and
-// 41, and 57 to 60 with an 8 bit form, so that other rows keep one chunk).
+// a time. Forward, 46 M values of bf16 in rows of 1025, 1501, 2047, 3001, 4095,
+// 5001, 6697 and 8191: 64, 49, 41, 50, 43, 63, 51 and 45 us halved, 79, 56, 47,
+// 63, 53, 84, 72 and 65 not; fp32 1 to 19 % less halved. Rows of 6696 take 42
+// us and 41, and 57 to 60 with an 8 bit form: even rows keep one chunk.
+// Backward, the other way about: 75, 61, 56, 62, 58, 82, 73 and 71 us with one
+// chunk, 88, 70, 60, 71, 64, 80, 72 and 68 with two, fp32 all slower by 1 to 9
+// %, since two chunks leave no registers for the next row's loads.
 template <bool HALVED, typename Fn>
 hipError_t by_width(int D, Fn fn) {
   const auto go = [&](auto odd) {
