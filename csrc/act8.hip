@@ -5,10 +5,10 @@
 // consecutive values of a row, so that a block of 64 is 8 neighbouring
 // lanes and its maximum costs three register permutations.
 //
-// Measured in bf16: 16384 x 2304 packed in 20 us (5.8 TB/s, some of it from
-// the last cache) and unpacked in 18 us, GELU of 16384 x 4096 forward with
-// both 8 bit forms in 70 us (5.8 TB/s), backward in 74 us (4.6 TB/s). GELU's
-// arithmetic takes about as long as its memory does.
+// Measured in bf16, calls of one kind in a row: 16384 x 2304 packed in 19 us
+// (5.9 TB/s, some of it from the last cache) and unpacked in 18 us, GELU of
+// 16384 x 4096 forward with both 8 bit forms in 75 us (5.4 TB/s), backward in
+// 63 us (5.4 TB/s). GELU's arithmetic takes about as long as its memory does.
 
 #include "act8.h"
 
