@@ -1,9 +1,10 @@
 """Modules of a transformer block that keep their activations in 8 bits.
 
-Drop-in subclasses of torch's, with the same parameters and state dict keys
-(checkpoints load either way), built on the operators of kfac_amd.ops. Each
-may hand the 8 bit form of its output to the next one, which then does not
-have to make it.
+Subclasses of torch's, with the same parameters and state dict keys
+(checkpoints load either way), built on the operators of kfac_amd.ops.
+Linear8 stands in for a linear layer as it is. LayerNorm8 and GELU8 return
+tuples: besides the result the 8 bit form of it, which the next linear layer
+then does not have to make, and LayerNorm8 the sum that it took the norm of.
 """
 
 from __future__ import annotations
