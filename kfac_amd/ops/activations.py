@@ -389,7 +389,8 @@ def linear8(
         check_packed(packed)
         check_same_shape(x, packed.codes, 'x and its packed form')
     dtype = x.dtype
-    if torch.is_autocast_enabled(x.device.type):
+    autocast = torch.is_autocast_enabled(x.device.type)
+    if autocast:
         dtype = torch.get_autocast_dtype(x.device.type)
         x = x.to(dtype)
     elif weight.dtype != dtype:
@@ -401,7 +402,9 @@ def linear8(
         weight.requires_grad or x.requires_grad
         or (bias is not None and bias.requires_grad)
     ):
-        # torch casts the bias itself under autocast only
-        return F.linear(x, weight, None if bias is None else bias.to(dtype))
+        # autocast casts 16 and 32 bit biases, and keeps the result
+        if bias is not None and not (autocast and bias.dtype in FLOAT_TYPES):
+            bias = bias.to(dtype)
+        return F.linear(x, weight, bias)
     codes, exps = packed if packed is not None else (None, None)
     return _Linear8.apply(x, weight, bias, codes, exps, dtype)

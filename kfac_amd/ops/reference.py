@@ -287,7 +287,7 @@ def weight_grad(
     g32 = g.to(torch.float32).reshape(-1, g.shape[-1])
     a32 = a.to(torch.float32).reshape(-1, a.shape[-1])
     db = g32.sum(0).to(bias_dtype) if bias else None
-    # which would multiply in its own type
+    # autocast would multiply in its own type
     with torch.autocast(g.device.type, enabled=False):
         dw = g32.t() @ a32
     return dw.to(dtype), db
